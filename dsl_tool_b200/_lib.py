@@ -19,13 +19,16 @@ LIB_PATH = os.environ.get("DSLGEMM_LIBRARY", os.path.join(_HERE, "libdslgemm.so"
 F32, BF16, F16 = 0, 1, 2
 FP8_PER_TENSOR, FP8_GROUP_1X128, FP8_BLOCK_128X128 = 0, 1, 2
 FP4_NV, FP4_MX = 0, 1
-OP_GEMM_FP8, OP_GEMM_BF16, OP_GEMM_FP4_NV, OP_GEMM_FP4_MX, OP_GEMM_FP8_GROUPWISE = 0, 1, 2, 3, 4
+OP_GEMM_FP8, OP_GEMM_BF16, OP_GEMM_FP4_NV, OP_GEMM_FP4_MX, OP_GEMM_FP8_GROUPWISE, OP_GEMM_INT8 = 0, 1, 2, 3, 4, 5
 ACT_NONE, ACT_SWIGLU, ACT_GEGLU = 0, 1, 2
 OUT_NVFP4 = 3
+NORM_NONE, NORM_INT8, NORM_FP8_GROUP_1X128, NORM_FP8_GIVEN = 0, 1, 2, 3
 MAX_GROUPS = 1024
 STATIC_SCRATCH_BYTES = 4 << 20
 WS_HEADER_BYTES = 64 << 10
 PER_TOKEN_MAX_COLS = 32768
+ROW_MAX_COLS = 32768
+INT8_MAX_K = 131056
 
 _ERR_NAMES = {
     -1: "a required pointer is NULL",
@@ -73,7 +76,7 @@ class Weight(ctypes.Structure):
     ]
 
 
-W_FP8, W_FP8_BLOCK128, W_NVFP4, W_MXFP4, W_BF16 = 0, 1, 2, 3, 4
+W_FP8, W_FP8_BLOCK128, W_NVFP4, W_MXFP4, W_BF16, W_INT8 = 0, 1, 2, 3, 4, 5
 
 _lib: Optional[ctypes.CDLL] = None
 _lock = threading.Lock()
@@ -86,9 +89,12 @@ _SIGNATURES = {
     "dsl_quant_fp8": (_i, [_vp, _i, _ll, _ll, _i, _vp, _i, _vp, _vp, _vp]),
     "dsl_quant_fp4": (_i, [_vp, _i, _ll, _ll, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     "dsl_quant_fp4_per_token": (_i, [_vp, _i, _ll, _ll, _vp, _vp, _vp, _vp, _i, _vp]),
+    "dsl_quant_int8": (_i, [_vp, _i, _ll, _ll, _vp, _vp, _vp]),
+    "dsl_rms_norm": (_i, [_vp, _i, _ll, _ll, _vp, _vp, _i, _f, _i, _vp, _vp, _vp, _vp, _vp]),
     "dsl_pack_kn": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, ctypes.c_size_t, _vp, _vp]),
     "dsl_transpose_u8": (_i, [_vp, _vp, _i, _i, _vp]),
     "dsl_gemm_fp8": (_i, [_vp, _vp, _vp, _ll, _ll, _i, _i, _vp, _i, ctypes.POINTER(Epilogue), _vp, _vp]),
+    "dsl_gemm_int8": (_i, [_vp, _vp, _vp, _ll, _ll, _i, _i, _vp, _i, ctypes.POINTER(Epilogue), _vp, _vp]),
     "dsl_gemm_fp8_groupwise": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _ll, _ll, _i, _i, _vp, _i,
                                     ctypes.POINTER(Epilogue), _vp, _vp]),
     "dsl_gemm_fp4": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _ll, _ll, _i, _i, _vp, _i,
@@ -100,6 +106,7 @@ _SIGNATURES = {
     "dsl_linear_scratch_bytes": (ctypes.c_size_t, [_i, _ll, _i, _i]),
     "dsl_linear": (_i, [_vp, _i, _ll, ctypes.POINTER(Weight), _vp, _vp, ctypes.c_size_t, _vp, _ll,
                         ctypes.POINTER(Epilogue), _vp, _vp]),
+    "dsl_linear_quantized": (_i, [_vp, _vp, _ll, ctypes.POINTER(Weight), _vp, _vp, _ll, ctypes.POINTER(Epilogue), _vp, _vp]),
     "dsl_quant_fp4_ref32": (_i, [_vp, _i, _ll, _vp, _vp, _vp]),
     "dsl_gemm_fp4_ref32": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "dsl_moe_route": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),

@@ -3,6 +3,7 @@
 
 #include "dslgemm.h"
 #include "gemm.cuh"
+#include "norm.cuh"
 #include "quant.cuh"
 
 using namespace dsl;
@@ -100,6 +101,31 @@ int dsl_quant_fp4(const void* x, int dtype, long long rows, long long cols, int 
 int dsl_quant_fp4_per_token(const void* x, int dtype, long long rows, long long cols, float* gs_out, uint8_t* q_out,
                             uint8_t* sf_out, const int* group_offsets, int groups, void* stream) {
     return quant_fp4_per_token_impl(x, dtype, rows, cols, gs_out, q_out, sf_out, group_offsets, groups, false, stream);
+}
+
+int dsl_quant_int8(const void* x, int dtype, long long rows, long long cols, float* scale_out, int8_t* q_out, void* stream) {
+    if (x == nullptr || scale_out == nullptr || q_out == nullptr) return DSL_ERR_NULL;
+    if (dtype < DSL_F32 || dtype > DSL_F16) return DSL_ERR_ENUM;
+    if (rows < 0 || cols < 0 || rows > 0x7FFFFFFFll || cols % 16 != 0) return DSL_ERR_SHAPE;
+    if (cols > DSL_ROW_MAX_COLS) return DSL_ERR_TOO_LARGE;
+    if (!aligned16(x) || !aligned16(q_out)) return DSL_ERR_ALIGN;
+    if (rows == 0 || cols == 0) return 0;
+    return static_cast<int>(launch_quant_int8(x, dtype, rows, static_cast<int>(cols), scale_out, q_out, as_stream(stream)));
+}
+
+int dsl_rms_norm(const void* x, int dtype, long long rows, long long cols, const void* residual, const void* gain, int gain_dtype,
+                 float eps, int out_format, void* sum_out, void* out, float* scale_out, const float* scale_in, void* stream) {
+    if (x == nullptr || gain == nullptr || out == nullptr || (residual != nullptr && sum_out == nullptr)) return DSL_ERR_NULL;
+    if (dtype < DSL_F32 || dtype > DSL_F16 || gain_dtype < DSL_F32 || gain_dtype > DSL_F16) return DSL_ERR_ENUM;
+    if (out_format < DSL_NORM_NONE || out_format > DSL_NORM_FP8_GIVEN) return DSL_ERR_ENUM;
+    if ((out_format == DSL_NORM_INT8 || out_format == DSL_NORM_FP8_GROUP_1X128) && scale_out == nullptr) return DSL_ERR_NULL;
+    if (out_format == DSL_NORM_FP8_GIVEN && scale_in == nullptr) return DSL_ERR_NULL;
+    if (rows < 0 || rows > 0x7FFFFFFFll || cols <= 0 || cols % 16 != 0) return DSL_ERR_SHAPE;
+    if (cols > DSL_ROW_MAX_COLS) return DSL_ERR_TOO_LARGE;
+    if (!aligned16(x) || !aligned16(residual) || !aligned16(gain) || !aligned16(sum_out) || !aligned16(out)) return DSL_ERR_ALIGN;
+    if (rows == 0) return 0;
+    return static_cast<int>(launch_rms_norm(x, dtype, rows, static_cast<int>(cols), residual, gain, gain_dtype, eps, out_format,
+                                            sum_out, out, scale_out, scale_in, as_stream(stream)));
 }
 
 int dsl_pack_kn(const void* w, int dtype, int groups, int K, int N, int format, int interleave, float* scale_io, int scale_given,
@@ -217,6 +243,18 @@ int dsl_gemm_bf16(const void* A, const void* B, void* C, long long ldc, long lon
     return launch_gemm(KIND_BF16, A, B, a, as_stream(stream));
 }
 
+int dsl_gemm_int8(const int8_t* A, const int8_t* B, void* C, long long ldc, long long M_total, int N, int K,
+                  const int* group_offsets, int groups, const dsl_epilogue* ep, uint32_t* status, void* stream) {
+    GemmArgs a;
+    if (K > DSL_INT8_MAX_K) return DSL_ERR_TOO_LARGE;
+    int rc = fill_common(a, A, B, C, ldc, M_total, N, K, group_offsets, groups, ep, status);
+    if (rc != 0) return rc;
+    if (a.b_kn) return DSL_ERR_ENUM;         // K-major weights only
+    a.scale_product = 0;
+    a.acc_int = 1;
+    return launch_gemm(KIND_I8, A, B, a, as_stream(stream));
+}
+
 int dsl_gemm_fp8_groupwise(const uint8_t* A, const uint8_t* B, const float* sa, const float* sb, int sb_block,
                            void* C, long long ldc, long long M_total, int N, int K, const int* group_offsets,
                            int groups, const dsl_epilogue* ep, uint32_t* status, void* stream) {
@@ -264,6 +302,7 @@ static bool problem_of(int op, long long M, int N, int K, int* kind, GemmArgs* a
         case DSL_OP_GEMM_FP4_NV: *kind = KIND_NVF4; k_bytes = K / 2; break;
         case DSL_OP_GEMM_FP4_MX: *kind = KIND_MXF4; k_bytes = K / 2; break;
         case DSL_OP_GEMM_FP8_GROUPWISE: *kind = KIND_F8G; k_bytes = K; break;
+        case DSL_OP_GEMM_INT8: *kind = KIND_I8; k_bytes = K; break;
         default: return false;                        // the quantisers use none
     }
     if (k_bytes <= 0 || k_bytes > 0x7FFFFFFFll) return false;

@@ -173,6 +173,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             if (KIND == KIND_NVF4) idesc |= (1u << 7) | (1u << 10);                 // e2m1 x e2m1, UE4M3 scales
             if (KIND == KIND_MXF4) idesc |= (1u << 7) | (1u << 10) | (1u << 23);    // e2m1 x e2m1, UE8M0 scales
             if (KIND == KIND_BF16) idesc |= (1u << 4) | (1u << 7) | (1u << 10);     // fp32 accumulate, bf16 x bf16
+            if (KIND == KIND_I8) idesc |= (2u << 4) | (1u << 7) | (1u << 10);       // int32 accumulate, int8 x int8
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -212,6 +213,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                             mma_f8f6f4(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_BF16) {
                             mma_f16(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, accum);
+                        } else if (KIND == KIND_I8) {
+                            mma_i8(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_NVF4) {
                             mma_nvf4(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, tmem_base + SFA_COL + k * 4,
                                      tmem_base + SFB_COL + k * (BLOCK_N / 32), accum);
@@ -259,6 +262,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                 if (split_k > 1) {
                     store_partial32(args, ks, row, col0, true, v);
                 } else {
+                    acc_values<KIND>(v);
                     store_chunk32(args, row, col0, ti.group, v, s1, s2, rs, vec_ok, ti.mtile, quad * 32 + lane);
                 }
             }
@@ -286,8 +290,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
 }
 
 
-// Sums the split-K partial products in slice order (deterministic) and applies the epilogue.
+// Sums the split-K partial products in slice order (deterministic) and applies the epilogue.  INT: int32 sums.
 // One thread per four consecutive columns of a row.
+template <bool INT>
 __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmArgs args, int split_k) {
     const int n4 = (args.n + 3) / 4;
     const long long id = blockIdx.x * 256ll + threadIdx.x;
@@ -297,6 +302,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmArgs args,
     float s1 = args.s1_dev != nullptr ? *args.s1_dev : args.s1;
     float s2 = args.s2_dev != nullptr ? *args.s2_dev : args.s2;
     if (args.scale_product) { s1 = s1 * s2; s2 = 1.0f; }
+    constexpr int SUM = INT ? KIND_I8 : KIND_F8;       // how the slices' sums are added
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     const size_t slice = static_cast<size_t>(args.m_total) * args.n;
     const float* p = args.partial + static_cast<size_t>(row) * args.n + col0;
@@ -310,18 +316,23 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmArgs args,
             v[ks] = ks < split_k ? __ldcg(reinterpret_cast<const float4*>(p + ks * slice)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-            if (ks < split_k) { acc[0] += v[ks].x; acc[1] += v[ks].y; acc[2] += v[ks].z; acc[3] += v[ks].w; }
+            if (ks < split_k) {
+                acc[0] = acc_add<SUM>(acc[0], v[ks].x);
+                acc[1] = acc_add<SUM>(acc[1], v[ks].y);
+                acc[2] = acc_add<SUM>(acc[2], v[ks].z);
+                acc[3] = acc_add<SUM>(acc[3], v[ks].w);
+            }
         }
     } else {
         for (int ks = 0; ks < split_k; ++ks, p += slice)
             for (int i = 0; i < 4; ++i)
-                if (col0 + i < args.n) acc[i] += p[i];
+                if (col0 + i < args.n) acc[i] = acc_add<SUM>(acc[i], p[i]);
     }
     const float rs = args.row_scale != nullptr ? args.row_scale[row] : 1.0f;
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        x[i] = __fmul_rn(__fmul_rn(acc[i], s1), s2);
+        x[i] = __fmul_rn(__fmul_rn(acc_value<SUM>(acc[i]), s1), s2);
         if (args.row_scale != nullptr) x[i] = __fmul_rn(x[i], rs);
         if (args.col_scale != nullptr && col0 + i < args.n) x[i] = __fmul_rn(x[i], args.col_scale[col0 + i]);
     }
@@ -469,7 +480,9 @@ static int launch_one(const void* A, const void* B, const GemmArgs& args, long l
 
 int launch_splitk_reduce(const GemmArgs& args, cudaStream_t st) {
     const long long threads = static_cast<long long>(args.m_total) * ((args.n + 3) / 4);
-    splitk_reduce_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, st>>>(args, args.split_k);
+    const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+    if (args.acc_int) splitk_reduce_kernel<true><<<blocks, 256, 0, st>>>(args, args.split_k);
+    else splitk_reduce_kernel<false><<<blocks, 256, 0, st>>>(args, args.split_k);
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -485,7 +498,7 @@ int choose_pair_split(int kind, const GemmArgs& args) {
     const long long tiles = ((args.m_total + 255ll) / 256) * ((args.n + 255ll) / 256);
     const int pairs = sm_count() / 2;
     if (pairs < 1 || tiles * 2 > pairs || num_kb < 8) return 1;
-    const double stage = kind == KIND_F8G ? 1200 : (kind == KIND_F8 ? 680 : 830);        // measured clocks per 128-byte K stage
+    const double stage = kind == KIND_F8G ? 1200 : (kind == KIND_F8 || kind == KIND_I8 ? 680 : 830);        // measured clocks per 128-byte K stage
     const double whole = static_cast<double>(num_kb) * stage;
     const size_t per_slice = static_cast<size_t>(args.m_total) * args.n * sizeof(float);
     size_t room = args.partial_bytes < (64u << 20) ? args.partial_bytes : (64u << 20);
@@ -603,6 +616,8 @@ int launch_gemm(int kind, const void* A, const void* B, GemmArgs args, cudaStrea
             return narrow ? launch_one<KIND_MXF4, 128>(A, B, args, max_tiles, st) : launch_one<KIND_MXF4, 256>(A, B, args, max_tiles, st);
         case KIND_BF16:
             return narrow ? launch_one<KIND_BF16, 128>(A, B, args, max_tiles, st) : launch_one<KIND_BF16, 256>(A, B, args, max_tiles, st);
+        case KIND_I8:
+            return narrow ? launch_one<KIND_I8, 128>(A, B, args, max_tiles, st) : launch_one<KIND_I8, 256>(A, B, args, max_tiles, st);
         default:
             return DSL_ERR_ENUM;
     }

@@ -10,12 +10,12 @@
 
 namespace dsl {
 
-enum { KIND_F8 = 0, KIND_NVF4 = 1, KIND_MXF4 = 2, KIND_BF16 = 3, KIND_F8G = 4 /* FP8 with fp32 scales per 128 K */ };
+enum { KIND_F8 = 0, KIND_NVF4 = 1, KIND_MXF4 = 2, KIND_BF16 = 3, KIND_F8G = 4 /* FP8 with fp32 scales per 128 K */, KIND_I8 = 5 /* int8, int32 sums */ };
 
 struct GemmArgs {
     int m_total;                 // rows of A / C over all row groups
     int n;                       // columns of C (rows of each group's weight)
-    int k_bytes;                 // bytes per operand row: K for FP8, K/2 for FP4, 2K for BF16
+    int k_bytes;                 // bytes per operand row: K for FP8 and INT8, K/2 for FP4, 2K for BF16
     int num_groups;
     const int* group_offsets;    // device int32[num_groups+1] row offsets, or nullptr (one group of m_total rows)
     const uint8_t* sfa;          // tiled block scales of A / B (FP4 kinds)
@@ -37,6 +37,7 @@ struct GemmArgs {
     int band;                    // column tiles per raster band (L2 reuse)
     int whole_tiles_only;        // 1: the tiles after the last full round are not cut into narrow pieces (measurements)
     int split_k;                 // > 1: K is cut into this many slices whose fp32 partial sums go to `partial`
+    int acc_int;                 // 1: accumulators and partial sums are int32 (KIND_I8), converted to fp32 where the scales are applied
     float* partial;              // [split_k, m_total, n] scratch (dense problems only): the caller's workspace
                                  // after its first DSL_WS_HEADER_BYTES
     size_t partial_bytes;        // capacity of `partial`

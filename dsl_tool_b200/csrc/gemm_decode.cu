@@ -289,6 +289,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         if (KIND == KIND_NVF4) idesc |= (1u << 7) | (1u << 10);
         if (KIND == KIND_MXF4) idesc |= (1u << 7) | (1u << 10) | (1u << 23);
         if (KIND == KIND_BF16) idesc |= (1u << 4) | (1u << 7) | (1u << 10);
+        if (KIND == KIND_I8) idesc |= (2u << 4) | (1u << 7) | (1u << 10);
         // weight given [K, N]: the M side is MN-major (bit 15), 32 bytes of K are 16 / 32 rows of 128 bytes
         const bool w_kn = C::SF_ATOMS == 0 && args.b_kn != 0;
         if (w_kn) idesc |= 1u << 15;
@@ -351,6 +352,8 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
                             mma_f8f6f4(d_tmem, wdesc + w_step * k, xdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_BF16) {
                             mma_f16(d_tmem, wdesc + w_step * k, xdesc + 2 * k, idesc, accum);
+                        } else if (KIND == KIND_I8) {
+                            mma_i8(d_tmem, wdesc + 2 * k, xdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_NVF4) {
                             mma_nvf4(d_tmem, wdesc + 2 * k, xdesc + 2 * k, idesc, tmem_base + DEC_SFW_COL + k * 4,
                                      tmem_base + DEC_SFX_COL + k * 4, accum);
@@ -468,14 +471,16 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll 1
                                 for (int p = 1; p < runs; ++p) {                   // ascending K
                                     const float4 pa = src[p * (TOK * 32)], pb = src[p * (TOK * 32) + 1];
-                                    a.x += pa.x; a.y += pa.y; a.z += pa.z; a.w += pa.w;
-                                    b.x += pb.x; b.y += pb.y; b.z += pb.z; b.w += pb.w;
+                                    a.x = acc_add<KIND>(a.x, pa.x); a.y = acc_add<KIND>(a.y, pa.y);
+                                    a.z = acc_add<KIND>(a.z, pa.z); a.w = acc_add<KIND>(a.w, pa.w);
+                                    b.x = acc_add<KIND>(b.x, pb.x); b.y = acc_add<KIND>(b.y, pb.y);
+                                    b.z = acc_add<KIND>(b.z, pb.z); b.w = acc_add<KIND>(b.w, pb.w);
                                 }
                                 float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
                                 const float rs = args.row_scale != nullptr ? args.row_scale[r] : 1.0f;
 #pragma unroll
                                 for (int j = 0; j < 8; ++j) {
-                                    x[j] = __fmul_rn(__fmul_rn(x[j], s1), s2);
+                                    x[j] = __fmul_rn(__fmul_rn(acc_value<KIND>(x[j]), s1), s2);
                                     if (args.row_scale != nullptr) x[j] = __fmul_rn(x[j], rs);
                                     if (args.col_scale != nullptr) x[j] = __fmul_rn(x[j], cs8[j]);
                                 }
@@ -568,7 +573,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int row = c * 4 + i;
-                        if (row < args.m_total) store_out(args, row, col, __uint_as_float(v[i]), s1, s2, cs, col_ok);
+                        if (row < args.m_total) store_out(args, row, col, acc_value<KIND>(__uint_as_float(v[i])), s1, s2, cs, col_ok);
                     }
                     __syncwarp();            // lanes leave store_out apart; the next load from tensor memory takes the whole warp
                 }
@@ -634,11 +639,11 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
                                 const int a = max(s_u0[c], t0);
                                 const float* src = args.partial + (static_cast<size_t>(dec_slot(s_u0, c, a)) * TOK + row0) * 128 + nl;
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) sum[j] += row0 + j < args.m_total ? __ldcg(src + j * 128) : 0.f;
+                                for (int j = 0; j < 4; ++j) sum[j] = acc_add<KIND>(sum[j], row0 + j < args.m_total ? __ldcg(src + j * 128) : 0.f);
                             }
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (row0 + j < args.m_total) store_out(args, row0 + j, col, sum[j], s1, s2, cs, col_ok);
+                                if (row0 + j < args.m_total) store_out(args, row0 + j, col, acc_value<KIND>(sum[j]), s1, s2, cs, col_ok);
                         }
                     }
                     if (warp == 2 && lane == 0) *reinterpret_cast<volatile unsigned long long*>(plan.arrivals + tile) = 0ull;
@@ -819,6 +824,7 @@ size_t decode_scratch_bytes(int kind, const GemmArgs& args, bool* served) {
         case KIND_MXF4: *served = plan_decode_kind<KIND_MXF4>(args, &wanted); break;
         case KIND_BF16: *served = plan_decode_kind<KIND_BF16>(args, &wanted); break;
         case KIND_F8G: *served = plan_decode_kind<KIND_F8G>(args, &wanted); break;
+        case KIND_I8: *served = plan_decode_kind<KIND_I8>(args, &wanted); break;
         default: break;
     }
     return *served ? wanted : 0;
@@ -842,6 +848,7 @@ int launch_gemm_decode(int kind, const void* A, const void* B, const GemmArgs& a
         case KIND_MXF4: return launch_decode_kind<KIND_MXF4>(A, B, args, st);
         case KIND_BF16: return launch_decode_kind<KIND_BF16>(A, B, args, st);
         case KIND_F8G: return launch_decode_kind<KIND_F8G>(A, B, args, st);
+        case KIND_I8: return launch_decode_kind<KIND_I8>(A, B, args, st);
         default: return DSL_ERR_ENUM;
     }
 }

@@ -219,6 +219,7 @@ gemm_decode_grouped_kernel(const __grid_constant__ CUtensorMap tmap_w, const __g
         if (KIND == KIND_NVF4) idesc |= (1u << 7) | (1u << 10);
         if (KIND == KIND_MXF4) idesc |= (1u << 7) | (1u << 10) | (1u << 23);
         if (KIND == KIND_BF16) idesc |= (1u << 4) | (1u << 7) | (1u << 10);
+        if (KIND == KIND_I8) idesc |= (2u << 4) | (1u << 7) | (1u << 10);
         // weight given [K, N]: the M side is MN-major (bit 15), 32 bytes of K are 16 / 32 rows of 128 bytes
         const bool w_kn = C::SF_ATOMS == 0 && args.b_kn != 0;
         if (w_kn) idesc |= 1u << 15;
@@ -255,6 +256,8 @@ gemm_decode_grouped_kernel(const __grid_constant__ CUtensorMap tmap_w, const __g
                             mma_f8f6f4(d_tmem, wdesc + w_step * k, xdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_BF16) {
                             mma_f16(d_tmem, wdesc + w_step * k, xdesc + 2 * k, idesc, accum);
+                        } else if (KIND == KIND_I8) {
+                            mma_i8(d_tmem, wdesc + 2 * k, xdesc + 2 * k, idesc, accum);
                         } else if (KIND == KIND_NVF4) {
                             mma_nvf4(d_tmem, wdesc + 2 * k, xdesc + 2 * k, idesc, tmem_base + dg::SFW_COL + k * 4,
                                      tmem_base + dg::SFX_COL + k * 4 + sf_col, accum);
@@ -335,6 +338,7 @@ gemm_decode_grouped_kernel(const __grid_constant__ CUtensorMap tmap_w, const __g
                     uint32_t v[32];
                     tmem_ld_32x32b_x32(tmem_lane + buf * TOK + c, v);
                     tmem_ld_wait();
+                    acc_values<KIND>(v);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) turn[i * 33 + lane] = __uint_as_float(v[i]);
                     if (c + 32 >= it.rows) {        // everything is out of tensor memory: the next but one item may have it
@@ -446,6 +450,7 @@ int launch_gemm_decode_grouped(int kind, const void* A, const void* B, const Gem
         case KIND_MXF4: return launch_grouped_kind<KIND_MXF4>(A, B, args, st);
         case KIND_BF16: return launch_grouped_kind<KIND_BF16>(A, B, args, st);
         case KIND_F8G: return launch_grouped_kind<KIND_F8G>(A, B, args, st);
+        case KIND_I8: return launch_grouped_kind<KIND_I8>(A, B, args, st);
         default: return DSL_ERR_ENUM;
     }
 }

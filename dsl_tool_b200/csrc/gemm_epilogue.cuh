@@ -12,6 +12,24 @@
 
 namespace dsl {
 
+// Accumulators are carried as 32-bit patterns: fp32, or int32 for the integer kind.  Integer partial sums are added as integers
+// (exact whatever the order) and converted once, where the scales are applied; the conversion rounds to 24 bits.
+template <int KIND>
+__device__ __forceinline__ float acc_add(float a, float b) {
+    return KIND == KIND_I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b;
+}
+template <int KIND>
+__device__ __forceinline__ float acc_value(float a) {
+    return KIND == KIND_I8 ? __int2float_rn(__float_as_int(a)) : a;
+}
+template <int KIND, int N>
+__device__ __forceinline__ void acc_values(uint32_t (&v)[N]) {
+    if (KIND == KIND_I8) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__int2float_rn(static_cast<int>(v[i])));
+    }
+}
+
 // One NVFP4 block of the result: 16 consecutive output columns of one row -> 8 packed bytes + one
 // scale byte in the tile layout, with the arithmetic of the NVFP4 quantiser (quant.cu):
 //   sf = ue4m3_rne(min((amax/6)/gs, 448)),  q = e2m1_rne(x * (1 / (f32(sf) * gs))).
@@ -62,7 +80,7 @@ __device__ __forceinline__ void scale32(const GemmArgs& args, const uint32_t (&v
     }
 }
 
-// Raw fp32 sums of K slice `ks` (32 columns of a row) to the split-K scratch; the reduction applies scales and activation.
+// Raw sums (fp32, or int32 of the integer kind) of K slice `ks` (32 columns of a row) to the split-K scratch; the reduction applies scales and activation.
 __device__ __forceinline__ void store_partial32(const GemmArgs& args, int ks, int row, int col0, bool row_ok, const uint32_t (&v)[32]) {
     if (!row_ok || col0 >= args.n) return;
     float* dst = args.partial + (static_cast<size_t>(ks) * args.m_total + row) * args.n + col0;

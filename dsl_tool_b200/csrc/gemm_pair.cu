@@ -252,6 +252,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             if (KIND == KIND_NVF4) idesc |= (1u << 7) | (1u << 10);
             if (KIND == KIND_MXF4) idesc |= (1u << 7) | (1u << 10) | (1u << 23);
             if (KIND == KIND_BF16) idesc |= (1u << 4) | (1u << 7) | (1u << 10);
+            if (KIND == KIND_I8) idesc |= (2u << 4) | (1u << 7) | (1u << 10);
             // B MN-major: bit 16 of the instruction descriptor, 32 bytes of K are 16 / 32 rows of 128 bytes
             const bool b_kn = C::SF_ATOMS == 0 && args.b_kn != 0;
             if (b_kn) idesc |= 1u << 16;
@@ -299,6 +300,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                                 mma_f8f6f4_pair(d_tmem, adesc + 2 * k, bdesc + b_step * k, idesc, accum);
                             } else if (KIND == KIND_BF16) {
                                 mma_f16_pair(d_tmem, adesc + 2 * k, bdesc + b_step * k, idesc, accum);
+                            } else if (KIND == KIND_I8) {
+                                mma_i8_pair(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, accum);
                             } else if (KIND == KIND_NVF4) {
                                 mma_nvf4_pair(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, tmem_base + pr::SFA_COL + k * 4,
                                               tmem_base + pr::SFB_COL + k * 8, accum);
@@ -377,6 +380,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(ovl_free, 0);
                 }
+                if constexpr (!SPLIT) acc_values<KIND>(va);
                 if constexpr (SPLIT)
                     store_partial32(args, ks, row, ti.n0 + ca * 32, row_ok, va);
                 else if (warp_store && ti.n0 + ca * 32 + 32 <= args.n)
@@ -385,6 +389,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     store_chunk32(args, row, ti.n0 + ca * 32, ti.group, va, s1, s2, rs, vec_ok, ti.sf_tile + static_cast<int>(rank), quad * 32 + lane);
                 tmem_ld_wait();
                 if (j + 2 < pr::TILE_N / 32) tmem_ld_32x32b_x32(t_row + (rot ? ((j + 8) & 7) : j + 2) * 32, va);
+                if constexpr (!SPLIT) acc_values<KIND>(vb);
                 if constexpr (SPLIT)
                     store_partial32(args, ks, row, ti.n0 + cb * 32, row_ok, vb);
                 else if (warp_store && ti.n0 + cb * 32 + 32 <= args.n)
@@ -483,6 +488,8 @@ int launch_gemm_pair(int kind, const void* A, const void* B, GemmArgs args, cuda
             return args.split_k > 1 ? launch_pair_one<KIND_MXF4, true>(A, B, args, max_tiles, st) : launch_pair_one<KIND_MXF4, false>(A, B, args, max_tiles, st);
         case KIND_BF16:
             return args.split_k > 1 ? launch_pair_one<KIND_BF16, true>(A, B, args, max_tiles, st) : launch_pair_one<KIND_BF16, false>(A, B, args, max_tiles, st);
+        case KIND_I8:
+            return args.split_k > 1 ? launch_pair_one<KIND_I8, true>(A, B, args, max_tiles, st) : launch_pair_one<KIND_I8, false>(A, B, args, max_tiles, st);
         default: return DSL_ERR_ENUM;
     }
 }

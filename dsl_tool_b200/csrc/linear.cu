@@ -40,6 +40,7 @@ bool carve(int format, long long M, int K, int groups, Carve* c) {
             c->scale_bytes = groups > 1 ? dsl_sf_bytes_grouped(M, K / 32, groups) : dsl_sf_bytes(M, K / 32);
             break;
         case DSL_W_BF16: c->q_bytes = 0; c->scale_bytes = 0; break;
+        case DSL_W_INT8: c->q_bytes = m * K; c->scale_bytes = m * sizeof(float); break;
         default: return false;
     }
     c->off_scale = align_up(c->q_bytes, 256);
@@ -100,6 +101,15 @@ extern "C" int dsl_linear(const void* x, int x_dtype, long long M, const dsl_wei
             return dsl_gemm_fp8_groupwise(qa, static_cast<const uint8_t*>(w->q), static_cast<const float*>(scales),
                                           static_cast<const float*>(w->scale), 1, C, ldc, M, w->n, w->k, offs, w->groups, &e,
                                           status, stream);
+        case DSL_W_INT8:
+            if (w->scale == nullptr) return DSL_ERR_NULL;
+            if (ep->row_scale != nullptr || ep->col_scale != nullptr) return DSL_ERR_ENUM;      // the two scales' own slots
+            rc = dsl_quant_int8(x, x_dtype, M, w->k, static_cast<float*>(scales), reinterpret_cast<int8_t*>(qa), stream);
+            if (rc != 0) return rc;
+            e.row_scale = static_cast<const float*>(scales);
+            e.col_scale = static_cast<const float*>(w->scale);
+            return dsl_gemm_int8(reinterpret_cast<const int8_t*>(qa), static_cast<const int8_t*>(w->q), C, ldc, M, w->n, w->k, offs,
+                                 w->groups, &e, status, stream);
         case DSL_W_NVFP4:
         case DSL_W_MXFP4: {
             if (w->scale == nullptr) return DSL_ERR_NULL;
@@ -140,6 +150,35 @@ extern "C" int dsl_linear(const void* x, int x_dtype, long long M, const dsl_wei
                                 static_cast<const uint8_t*>(w->scale), fmt, C, ldc, M, w->n, w->k, offs, w->groups, &e, status,
                                 stream);
         }
+        default:
+            return DSL_ERR_ENUM;
+    }
+}
+
+extern "C" int dsl_linear_quantized(const void* q, const float* q_scale, long long M, const dsl_weight* w, const int* group_offsets,
+                                    void* C, long long ldc, const dsl_epilogue* ep, uint32_t* status, void* stream) {
+    if (q == nullptr || q_scale == nullptr || w == nullptr || C == nullptr || ep == nullptr || w->q == nullptr || w->scale == nullptr)
+        return DSL_ERR_NULL;
+    if (w->groups < 1 || w->n <= 0 || w->k <= 0) return DSL_ERR_SHAPE;
+    if (w->groups > 1 && group_offsets == nullptr) return DSL_ERR_NULL;
+    const int* offs = w->groups > 1 ? group_offsets : nullptr;
+    const float* w_scale = static_cast<const float*>(w->scale);
+    dsl_epilogue e = *ep;
+    switch (w->format) {
+        case DSL_W_FP8:
+            e.scale_a_dev = q_scale;
+            e.scale_b_dev = w_scale;
+            return dsl_gemm_fp8(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(w->q), C, ldc, M, w->n, w->k, offs, w->groups,
+                                &e, status, stream);
+        case DSL_W_FP8_BLOCK128:
+            return dsl_gemm_fp8_groupwise(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(w->q), q_scale, w_scale, 1, C, ldc, M,
+                                          w->n, w->k, offs, w->groups, &e, status, stream);
+        case DSL_W_INT8:
+            if (ep->row_scale != nullptr || ep->col_scale != nullptr) return DSL_ERR_ENUM;      // the two scales' own slots
+            e.row_scale = q_scale;
+            e.col_scale = w_scale;
+            return dsl_gemm_int8(static_cast<const int8_t*>(q), static_cast<const int8_t*>(w->q), C, ldc, M, w->n, w->k, offs, w->groups,
+                                 &e, status, stream);
         default:
             return DSL_ERR_ENUM;
     }

@@ -1,0 +1,281 @@
+// Row-wise kernels that end in 8 bits: the root-mean-square norm with the residual's addition, and the int8 quantiser (the same
+// kernel without the norm).
+//
+//   t = round(x + r) to the type of x          (r optional; t is written, and is what the norm reads)
+//   y = (t * rsqrt(mean(t^2) + eps)) * w       in fp32, sum of squares in fp32
+//   int8:        s = max(amax_row |y| / 127, 1e-12),  q = rne(y / s)
+//   FP8 1x128:   s = max(amax_128 |y| / 448, 1e-12),  q = e4m3(y / s)
+//   FP8 given:   q = e4m3(y / s) with the caller's s
+//   none:        y in the type of x
+// q and s are those of the stand-alone quantisers on the fp32 y, bit for bit (quotients are correctly rounded).
+//
+// Bound by memory: x, r and w are read once, t, q and s written once (8192 x 8192 bf16 with residual: 403 MB).  One CTA takes a
+// row and keeps it in registers, 16 consecutive elements a thread, so the three looks at it (sum of squares, maximum, conversion)
+// cost one trip to memory; a CTA has as many threads as the row has 16-element pieces (a row of 4096: 256 threads, eight rows an
+// SM in flight), and rows beyond 1024 pieces give every thread two.  The two sums over a row are a shuffle tree and one meeting
+// in shared memory each; other CTAs of the SM cover it.
+//
+// A NaN anywhere in a row makes an int8 row's scale NaN (an integer cannot carry it): the maximum is taken over the bit patterns
+// of |y|, where every NaN is above infinity.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dslgemm.h"
+#include "norm.cuh"
+#include "ptx.cuh"
+#include "quant_math.cuh"
+
+namespace dsl {
+
+enum { ROW_NONE = 0, ROW_INT8 = 1, ROW_FP8_GROUP = 2, ROW_FP8_GIVEN = 3 };
+
+struct RowArgs {
+    const void* x;
+    const void* residual;      // type of x, or nullptr
+    const void* gain;          // [cols]
+    int gain_dtype;
+    void* sum_out;             // x + residual, type of x (only with a residual)
+    void* out;                 // int8 / E4M3 bytes, or the type of x
+    float* scale_out;          // int8 [rows]; FP8 1x128 [rows, ceil(cols / 128)]
+    const float* scale_in;     // FP8 given: one float
+    float eps;
+    int cols;
+    bool wide;                 // rows of x, residual and sum start on 32-byte boundaries
+};
+
+// 16 elements to global memory in the type of x.
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
+    if (sizeof(T) == 4) {
+        float4* d = reinterpret_cast<float4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (dsl_is_half<T>::value) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        uint4* d = reinterpret_cast<uint4*>(p);
+        d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+template <typename T> __device__ __forceinline__ float round_to(float v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ float round_to<__nv_bfloat16>(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+template <> __device__ __forceinline__ float round_to<__half>(float v) { return __half2float(__float2half_rn(v)); }
+
+__device__ __forceinline__ void load_gain(const void* gain, int dtype, int at, float (&w)[16]) {
+    if (dtype == DSL_F32) load16<float>(static_cast<const float*>(gain) + at, w);
+    else if (dtype == DSL_BF16) load16<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(gain) + at, w);
+    else load16<__half>(static_cast<const __half*>(gain) + at, w);
+}
+
+// 16 quotients y / s to the nearest whole numbers (ties to even), packed.  |y / s| <= 127 by the scale's definition (or everything
+// is NaN or divided by infinity: the conversion gives 0).
+__device__ __forceinline__ uint4 quant16_int8(const float (&v)[16], float s) {
+    const float inv = __frcp_rn(s), ns = -s;
+    unsigned long long inv2, neg_s2;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(inv2) : "f"(inv));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(neg_s2) : "f"(ns));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float f[4];
+        div2_for_e4m3<false>(v[4 * i], v[4 * i + 1], neg_s2, inv2, f[0], f[1]);
+        div2_for_e4m3<false>(v[4 * i + 2], v[4 * i + 3], neg_s2, inv2, f[2], f[3]);
+        const uint32_t lo = __byte_perm(__float2int_rn(f[0]), __float2int_rn(f[1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float2int_rn(f[2]), __float2int_rn(f[3]), 0x0040);
+        w[i] = __byte_perm(lo, hi, 0x5410);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// max(amax / 127, 1e-12), one IEEE division; a NaN stays one.
+__device__ __forceinline__ float int8_scale_from_amax(float amax) {
+    const float s = __fdiv_rn(amax, 127.0f);
+    return s < 1e-12f ? 1e-12f : s;
+}
+
+// All threads of the block: the sum / the largest bit pattern over the block.  `slots`: 32 words of its own for each call, so that
+// one barrier a call is enough.
+__device__ __forceinline__ float block_sum(float v, float* slots) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps == 1) return v;
+    if (lane == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? slots[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
+    v = __reduce_max_sync(0xFFFFFFFFu, v);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps == 1) return v;
+    if (lane == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return __reduce_max_sync(0xFFFFFFFFu, lane < warps ? slots[lane] : 0u);
+}
+
+// PIECES: 16-element pieces a thread holds; piece p of thread i starts at (p * blockDim.x + i) * 16.
+template <typename T, int OUT, bool NORM, int PIECES>
+__global__ void __launch_bounds__(1024) row_kernel(const RowArgs a) {
+    __shared__ float s_sum[32];
+    __shared__ uint32_t s_max[32];
+    // Launched as a dependent: placed while the kernel before it drains.  What follows may do the same once that one is complete.
+    griddep_wait();
+    griddep_launch_dependents();
+    const size_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.cols;
+    float v[PIECES][16];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int at = (p * blockDim.x + threadIdx.x) * 16;
+        if (at < a.cols) {
+            load16w<T>(x + at, v[p], a.wide);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[p][i] = 0.f;
+        }
+    }
+    if (NORM) {
+        float squares = 0.f;
+        if (a.residual != nullptr) {
+            const T* r = static_cast<const T*>(a.residual) + row * a.cols;
+            T* t = static_cast<T*>(a.sum_out) + row * a.cols;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const int at = (p * blockDim.x + threadIdx.x) * 16;
+                if (at >= a.cols) break;
+                float b[16];
+                load16w<T>(r + at, b, a.wide);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[p][i] = round_to<T>(__fadd_rn(v[p][i], b[i]));
+                store16<T>(t + at, v[p]);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) squares = fmaf(v[p][i], v[p][i], squares);
+        squares = block_sum(squares, s_sum);
+        const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares, static_cast<float>(a.cols)), a.eps));
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int at = (p * blockDim.x + threadIdx.x) * 16;
+            if (at >= a.cols) break;
+            float w[16];
+            load_gain(a.gain, a.gain_dtype, at, w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[p][i] = __fmul_rn(__fmul_rn(v[p][i], inv), w[i]);
+        }
+    }
+    uint8_t* q = static_cast<uint8_t*>(a.out) + row * a.cols;
+    float s = 0.f;
+    if (OUT == ROW_INT8) {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
+        s = int8_scale_from_amax(__uint_as_float(block_max(m, s_max)));
+        if (threadIdx.x == 0) a.scale_out[row] = s;
+    }
+    if (OUT == ROW_FP8_GIVEN) s = *a.scale_in;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int at = (p * blockDim.x + threadIdx.x) * 16;
+        if (OUT == ROW_FP8_GROUP) {      // eight neighbouring threads hold a group; threads past the row's end hold zeros
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[p][i]));
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            s = fp8_scale_from_amax(m);
+            if (at < a.cols && (threadIdx.x & 7) == 0) a.scale_out[row * ((a.cols + 127) / 128) + at / 128] = s;
+        }
+        if (at < a.cols) {
+            if (OUT == ROW_NONE) store16<T>(static_cast<T*>(a.out) + row * a.cols + at, v[p]);
+            else if (OUT == ROW_INT8) *reinterpret_cast<uint4*>(q + at) = quant16_int8(v[p], s);
+            else *reinterpret_cast<uint4*>(q + at) = quant16_e4m3<OUT == ROW_FP8_GIVEN>(v[p], s);
+        }
+    }
+}
+
+template <typename T, int OUT, bool NORM>
+static cudaError_t launch_row(const RowArgs& a, long long rows, cudaStream_t st) {
+    const int pieces = a.cols / 16;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows));
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (pieces <= 1024) {
+        cfg.blockDim = dim3((pieces + 31) / 32 * 32);
+        return cudaLaunchKernelEx(&cfg, row_kernel<T, OUT, NORM, 1>, a);
+    }
+    cfg.blockDim = dim3(((pieces + 1) / 2 + 31) / 32 * 32);
+    return cudaLaunchKernelEx(&cfg, row_kernel<T, OUT, NORM, 2>, a);
+}
+
+template <typename T>
+static cudaError_t launch_type(const RowArgs& a, int format, bool norm, long long rows, cudaStream_t st) {
+    if (!norm) return launch_row<T, ROW_INT8, false>(a, rows, st);
+    switch (format) {
+        case ROW_INT8: return launch_row<T, ROW_INT8, true>(a, rows, st);
+        case ROW_FP8_GROUP: return launch_row<T, ROW_FP8_GROUP, true>(a, rows, st);
+        case ROW_FP8_GIVEN: return launch_row<T, ROW_FP8_GIVEN, true>(a, rows, st);
+        default: return launch_row<T, ROW_NONE, true>(a, rows, st);
+    }
+}
+
+static cudaError_t launch_dtype(RowArgs& a, int dtype, int format, bool norm, long long rows, cudaStream_t st) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual);
+    a.wide = (all & 31u) == 0;           // a row is a multiple of 16 elements, i.e. of 32 bytes
+    if (dtype == DSL_F32) return launch_type<float>(a, format, norm, rows, st);
+    if (dtype == DSL_BF16) return launch_type<__nv_bfloat16>(a, format, norm, rows, st);
+    return launch_type<__half>(a, format, norm, rows, st);
+}
+
+cudaError_t launch_quant_int8(const void* x, int dtype, long long rows, int cols, float* scale_out, int8_t* q, cudaStream_t st) {
+    RowArgs a{};
+    a.x = x;
+    a.out = q;
+    a.scale_out = scale_out;
+    a.cols = cols;
+    return launch_dtype(a, dtype, ROW_INT8, false, rows, st);
+}
+
+cudaError_t launch_rms_norm(const void* x, int dtype, long long rows, int cols, const void* residual, const void* gain, int gain_dtype,
+                            float eps, int out_format, void* sum_out, void* out, float* scale_out, const float* scale_in,
+                            cudaStream_t st) {
+    RowArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.gain = gain;
+    a.gain_dtype = gain_dtype;
+    a.sum_out = sum_out;
+    a.out = out;
+    a.scale_out = scale_out;
+    a.scale_in = scale_in;
+    a.eps = eps;
+    a.cols = cols;
+    static_assert(ROW_NONE == DSL_NORM_NONE && ROW_INT8 == DSL_NORM_INT8 && ROW_FP8_GROUP == DSL_NORM_FP8_GROUP_1X128 &&
+                  ROW_FP8_GIVEN == DSL_NORM_FP8_GIVEN, "the header's codes");
+    return launch_dtype(a, dtype, out_format, true, rows, st);
+}
+
+}  // namespace dsl

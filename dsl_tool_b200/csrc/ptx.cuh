@@ -169,6 +169,14 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t adesc, uint64_t bde
         ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// int8 operands, int32 accumulators (wrap-around, never saturating: the host bounds K so that they cannot overflow)
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // e2m1 operands, one unsigned-E4M3 scale per 16 K-elements (4 scales per row per K=64 MMA).
 __device__ __forceinline__ void mma_nvf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
@@ -286,6 +294,7 @@ __device__ __forceinline__ void tc_cp_32x128b_warpx4_pair(uint32_t taddr, uint64
     }
 DSL_MMA_PAIR(mma_f8f6f4_pair, "f8f6f4")
 DSL_MMA_PAIR(mma_f16_pair, "f16")
+DSL_MMA_PAIR(mma_i8_pair, "i8")
 #undef DSL_MMA_PAIR
 __device__ __forceinline__ void mma_nvf4_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                               uint32_t sfa, uint32_t sfb, uint32_t accumulate) {

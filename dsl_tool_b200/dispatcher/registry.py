@@ -37,6 +37,9 @@ def _gemm_input_schema(kernel_name: str) -> dict:
         schema["scale_b"] = "float"
         schema["mode"] = "str: per_tensor | groupwise | block128 (default per_tensor)"
         schema["group_size"] = "int: K elements per scale, a multiple of 128 (default 128; other sizes only with already-quantised operands)"
+    if "int8" in kernel_name:
+        schema["scale_a"] = "Tensor[M] fp32 or float (already-quantised operands only)"
+        schema["scale_b"] = "Tensor[N] fp32 or float (already-quantised operands only)"
     if "fp4" in kernel_name:
         schema["scale_a"] = "Tensor uint8 (tiled block scales; packed operands only)"
         schema["scale_b"] = "Tensor uint8 (tiled block scales; packed operands only)"
@@ -45,7 +48,7 @@ def _gemm_input_schema(kernel_name: str) -> dict:
     if "grouped" in kernel_name:
         schema["num_groups"] = "int"
         schema["expert_offsets"] = "Tensor[G+1] int32 (ragged groups; optional)"
-        schema["format"] = "str: bf16 | fp8 | fp8_groupwise | nvfp4 | mxfp4 (default bf16)"
+        schema["format"] = "str: bf16 | fp8 | fp8_groupwise | int8 | nvfp4 | mxfp4 (default bf16)"
     if "bf16" not in kernel_name:
         schema["b_layout"] = "str: kn | nk (default kn)"
         schema["out_dtype"] = "str: float32 | bfloat16"
@@ -94,6 +97,7 @@ class KernelRegistry:
         table = [
             ("gemm.fp8_gemm", k.fp8_gemm, "FP8 E4M3 GEMM with per-tensor or 128-group scaling (tcgen05, sm_100a)"),
             ("gemm.fp4_gemm", k.fp4_gemm, "Block-scaled FP4 GEMM: NVFP4 / MXFP4 (tcgen05, sm_100a)"),
+            ("gemm.int8_gemm", k.int8_gemm, "INT8 GEMM with a scale per token and per output channel, exact int32 sums (tcgen05, sm_100a)"),
             ("gemm.grouped_gemm", k.grouped_gemm, "Grouped / batched GEMM for MoE / LoRA, fixed or ragged groups"),
             ("gemm.bf16_gemm", k.bf16_gemm, "BF16 GEMM (A[M,K] @ B[K,N]), fp32 accumulate"),
         ]

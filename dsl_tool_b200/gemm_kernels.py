@@ -17,7 +17,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .quantize import PackedWeight, _pack_kn, _pack_kn_serves, pack_weight, quantize_fp4, quantize_fp8, transpose_bytes
+from .quantize import PackedWeight, _pack_kn, _pack_kn_serves, pack_weight, quantize_fp4, quantize_fp8, quantize_int8, transpose_bytes
 from .weight_store import cached_pack
 
 _FLOAT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -222,6 +222,43 @@ def gemm_fp8_groupwise_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, sa: torc
     return out
 
 
+def gemm_int8_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, scale_a: Scalar, scale_b: Scalar, *, n: int,
+                        out_dtype=torch.float32, expert_offsets: Optional[torch.Tensor] = None, b_static: bool = False,
+                        activation: Optional[str] = None, out_global_scale: Scalar = None):
+    """C = (qa @ qb^T) * scale_a * scale_b on int8 operands, sums exact in int32; qa [M, K], qb_nk [G*N, K].  scale_a: fp32 [M], one
+    per token, or a scalar; scale_b: fp32 [G*N], one per output channel, or a scalar (a one-element tensor is a scalar).
+    `b_static` as in gemm_fp8_quantized."""
+    dev = _lib.require_cuda(qa, qb_nk)
+    if qa.dtype != torch.int8 or qb_nk.dtype != torch.int8:
+        raise TypeError(f"int8 operands are needed, got {qa.dtype} and {qb_nk.dtype}")
+    qa, qb_nk = qa.contiguous(), qb_nk.contiguous()
+    M, K = qa.shape
+    if K > _lib.INT8_MAX_K:
+        raise ValueError(f"K must be at most {_lib.INT8_MAX_K} (int32 sums), got {K}")
+    offs, groups = _offsets_arg(expert_offsets, dev)
+    if qb_nk.shape != (groups * n, K):
+        raise ValueError(f"weight must be [{groups}*{n}, {K}] int8, got {tuple(qb_nk.shape)}")
+    row_scale, scale_a = _vector_or_scalar(scale_a, M, "scale_a")
+    col_scale, scale_b = _vector_or_scalar(scale_b, groups * n, "scale_b")
+    nc = _out_cols(n, activation)
+    keep: list = []
+    ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation)
+    out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+    rc = _run(dev, ep, (_lib.OP_GEMM_INT8, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_int8(
+        qa.data_ptr(), qb_nk.data_ptr(), out.data_ptr(), ldc, M, n, K, _lib.ptr(offs), groups, ctypes.byref(ep), status, stream))
+    _lib.check(rc, "dsl_gemm_int8")
+    return ret
+
+
+def _vector_or_scalar(s: Scalar, count: int, name: str) -> Tuple[Optional[torch.Tensor], Scalar]:
+    """(per-row or per-column scales, scalar): exactly one of them is what `s` is."""
+    if not isinstance(s, torch.Tensor) or s.numel() == 1:
+        return None, s
+    if s.numel() != count:
+        raise ValueError(f"{name} must hold 1 or {count} values, got {tuple(s.shape)}")
+    return s.reshape(-1), None
+
+
 def gemm_fp4_quantized(pa: torch.Tensor, pb_nk: torch.Tensor, sfa: torch.Tensor, sfb: torch.Tensor, *,
                        format: str, n: int, global_scale_a: Scalar = None, global_scale_b: Scalar = None,
                        out_dtype=torch.float32, expert_offsets: Optional[torch.Tensor] = None,
@@ -291,12 +328,19 @@ def gemm_bf16_raw(a: torch.Tensor, b_nk: torch.Tensor, *, n: int, out_dtype=torc
 # quantise-and-multiply on one packed weight (shared by the public callables)
 # --------------------------------------------------------------------------------------
 
-_W_CODES = {"fp8": _lib.W_FP8, "fp8_block128": _lib.W_FP8_BLOCK128, "nvfp4": _lib.W_NVFP4, "mxfp4": _lib.W_MXFP4, "bf16": _lib.W_BF16}
+_W_CODES = {"fp8": _lib.W_FP8, "fp8_block128": _lib.W_FP8_BLOCK128, "nvfp4": _lib.W_NVFP4, "mxfp4": _lib.W_MXFP4, "bf16": _lib.W_BF16,
+            "int8": _lib.W_INT8}
 _OP_OF_FORMAT = {"fp8": _lib.OP_GEMM_FP8, "fp8_block128": _lib.OP_GEMM_FP8_GROUPWISE, "nvfp4": _lib.OP_GEMM_FP4_NV,
-                 "mxfp4": _lib.OP_GEMM_FP4_MX, "bf16": _lib.OP_GEMM_BF16}
+                 "mxfp4": _lib.OP_GEMM_FP4_MX, "bf16": _lib.OP_GEMM_BF16, "int8": _lib.OP_GEMM_INT8}
 
 
 def _new_weight_desc(w: PackedWeight) -> "_lib.Weight":
+    if w.format == "int8":      # read by pointer: an assembled weight has to be what pack_weight makes
+        s = w.scale
+        if w.q.dtype != torch.int8 or w.q.numel() != w.groups * w.n * w.k or not w.q.is_contiguous():
+            raise ValueError(f"an int8 weight holds contiguous int8 [{w.groups}*{w.n}, {w.k}], got {w.q.dtype} {tuple(w.q.shape)}")
+        if s is None or s.dtype != torch.float32 or s.numel() != w.groups * w.n or not s.is_contiguous() or s.device != w.q.device:
+            raise ValueError(f"an int8 weight needs {w.groups * w.n} contiguous float32 channel scales beside it")
     d = _lib.Weight()
     d.format, d.groups, d.n, d.k = _W_CODES[w.format], w.groups, w.n, w.k
     d.q = w.q.data_ptr()
@@ -326,6 +370,8 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
         if w.k > _lib.PER_TOKEN_MAX_COLS:
             raise ValueError(f"per-token scales need K <= {_lib.PER_TOKEN_MAX_COLS}")
         act_global_scale = None
+    if w.format == "int8" and (row_scale is not None or col_scale is not None):
+        raise ValueError("an int8 weight's scales occupy the row_scale and col_scale slots")
     """Quantise + GEMM through the single C entry point `dsl_linear`: one call into the library, the quantised
     activations in a per-stream arena instead of fresh allocations."""
     dev = a.device
@@ -383,9 +429,44 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
     return ret
 
 
+def _linear_quantized(a: torch.Tensor, act_scale: torch.Tensor, w: PackedWeight, out_dtype, expert_offsets, row_scale, col_scale,
+                      activation: Optional[str], out_global_scale: Scalar, act_global_scale: Scalar):
+    """`linear` on activations in the weight's format: the GEMM alone, one call into the library."""
+    fmt = w.format
+    if fmt not in ("fp8", "fp8_block128", "int8"):
+        raise ValueError(f"act_scale goes with FP8 and int8 weights, not {fmt}")
+    if act_global_scale is not None:
+        raise ValueError("act_scale and act_global_scale exclude each other")
+    if fmt == "int8" and (row_scale is not None or col_scale is not None):
+        raise ValueError("an int8 weight's scales occupy the row_scale and col_scale slots")
+    dev = _lib.require_cuda(a, act_scale, w.q, expert_offsets)
+    if (a.dtype != torch.int8) if fmt == "int8" else (a.dtype not in _BYTE_DTYPES):
+        raise TypeError(f"act_scale says that the activations are quantised for {fmt}, but they are {a.dtype}")
+    M, K = a.shape
+    want = 1 if fmt == "fp8" else M if fmt == "int8" else M * ((K + 127) // 128)
+    if act_scale.numel() != want:
+        raise ValueError(f"act_scale must hold {want} values for {M} rows of {fmt}, got {tuple(act_scale.shape)}")
+    a = a.contiguous()
+    act_scale = act_scale.detach().to(torch.float32).contiguous()
+    offs = None
+    if expert_offsets is not None:
+        offs, groups = _offsets_arg(expert_offsets, dev)
+        if groups != w.groups:
+            raise ValueError(f"expert_offsets describes {groups} groups, the weight holds {w.groups}")
+    desc = _weight_desc(w)
+    keep: list = []
+    ep = _epilogue(dev, None, None, None, row_scale, col_scale, keep, False, activation)
+    out, ldc, ret = _make_output(dev, M, _out_cols(w.n, activation), out_dtype, out_global_scale, offs, w.groups, ep, keep)
+    rc = _run(dev, ep, (_OP_OF_FORMAT[fmt], M, w.n, K, w.groups), lambda status, stream: _lib.lib().dsl_linear_quantized(
+        a.data_ptr(), act_scale.data_ptr(), M, ctypes.byref(desc), _lib.ptr(offs), out.data_ptr(), ldc, ctypes.byref(ep), status, stream))
+    _lib.check(rc, "dsl_linear_quantized")
+    return ret
+
+
 def linear(a: torch.Tensor, w: PackedWeight, *, out_dtype=torch.float32,
            expert_offsets: Optional[torch.Tensor] = None, row_scale=None, col_scale=None,
-           activation: Optional[str] = None, out_global_scale: Scalar = None, act_global_scale: Scalar = None):
+           activation: Optional[str] = None, out_global_scale: Scalar = None, act_global_scale: Scalar = None,
+           act_scale: Optional[torch.Tensor] = None):
     """a [M, K] high-precision activations x packed weight -> [M, N]: quantise the activations
     in the weight's format (one pass on the GPU) and run the matching GEMM.  A weight of a
     quantised format may be fetched while the activation quantiser still runs (which stands between the weight's
@@ -397,7 +478,9 @@ def linear(a: torch.Tensor, w: PackedWeight, *, out_dtype=torch.float32,
     (packed bytes, scale tiles, global scale), the A operand of a following `gemm_fp4_quantized`.
     `act_global_scale` (NVFP4 weights): the fp32 global scale of the activations, a float or a device scalar - a
     calibrated value instead of amax(a) / 2688 - or "per_token": one dynamic global scale per row (amax_row / 2688).
-    Either way the quantiser reads `a` once instead of twice (no tensor-wide amax pass)."""
+    Either way the quantiser reads `a` once instead of twice (no tensor-wide amax pass).
+    `act_scale` (FP8 and int8 weights): `a` is quantised already in the weight's format - by `rms_norm`, `quantize_fp8` or
+    `quantize_int8` - and these are its scales: one float ("fp8"), [M, K/128] ("fp8_block128") or [M] ("int8")."""
     if _activation_code(activation) != _lib.ACT_NONE and not w.gate_up_interleaved:
         raise ValueError("a gated activation needs a weight packed with gate_up_interleave=True")
     if a.dim() != 2 or a.shape[1] != w.k:
@@ -406,6 +489,9 @@ def linear(a: torch.Tensor, w: PackedWeight, *, out_dtype=torch.float32,
         raise ValueError("a multi-group weight needs expert_offsets")
     if _is_nvfp4_out(out_dtype) and w.format == "fp8_block128":
         raise ValueError("a quantised result is not available from the group-scaled FP8 GEMM")
+    if act_scale is not None:
+        return _linear_quantized(a, act_scale, w, out_dtype, expert_offsets, row_scale, col_scale, activation, out_global_scale,
+                                 act_global_scale)
     if (a.is_cuda and a.is_contiguous() and w.q.device == a.device and (w.groups > 1) == (expert_offsets is not None)
             and (a.dtype == torch.bfloat16 if w.format == "bf16" else a.dtype in _FLOAT_DTYPES)):
         offs = None
@@ -416,6 +502,12 @@ def linear(a: torch.Tensor, w: PackedWeight, *, out_dtype=torch.float32,
         return _linear_one_call(a, w, out_dtype, offs, row_scale, col_scale, activation, out_global_scale, act_global_scale)
     if act_global_scale is not None and w.format != "nvfp4":
         raise ValueError("act_global_scale applies to NVFP4 weights")
+    if w.format == "int8":
+        if row_scale is not None or col_scale is not None:
+            raise ValueError("an int8 weight's scales occupy the row_scale and col_scale slots")
+        qa, sa = quantize_int8(a)
+        return gemm_int8_quantized(qa, w.q, sa, w.scale, n=w.n, out_dtype=out_dtype, expert_offsets=expert_offsets, activation=activation,
+                                   out_global_scale=out_global_scale, b_static=True)
     common = dict(n=w.n, out_dtype=out_dtype, expert_offsets=expert_offsets, activation=activation)
     if _is_nvfp4_out(out_dtype):
         common["out_global_scale"] = out_global_scale
@@ -615,6 +707,50 @@ def _fp4_gemm_ref32(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
     return out
 
 
+def int8_gemm(A: torch.Tensor, B, scale_a: Scalar = None, scale_b: Scalar = None, *, b_layout: str = "kn", out_dtype="float32",
+              cache_weights: bool = False) -> torch.Tensor:
+    """INT8 GEMM, C[M,N] = (A[M,K] @ B[K,N]) * scale_a * scale_b with exact int32 sums (no counterpart in the reference; arguments
+    as fp8_gemm's).
+
+    * A and B int8: `scale_a` fp32 [M] (one per token), `scale_b` fp32 [N] (one per output channel); either may be a scalar.
+    * A and B high-precision: quantised on the GPU first, A with a scale per row, B with one per output channel.
+    * B a PackedWeight of format "int8": A high-precision, or int8 with `scale_a`.
+    b_layout "kn" is the reference's B[K,N] (transposed first), "nk" a K-major weight.  `cache_weights` as in fp8_gemm.
+    """
+    if b_layout not in ("kn", "nk"):
+        raise ValueError("b_layout must be 'kn' or 'nk'")
+    _lib.require_cuda(A, B if isinstance(B, torch.Tensor) else None)
+    if A.dim() != 2:
+        raise ValueError(f"A must be [M, K], got {tuple(A.shape)}")
+    if isinstance(B, PackedWeight):
+        if B.format != "int8" or B.groups != 1 or B.k != A.shape[1]:
+            raise ValueError(f"packed weight is {B.format} [{B.n},{B.k}], need single-group int8 with K={A.shape[1]}")
+        if scale_b is not None:
+            raise ValueError("a packed weight brings its own scales")
+        if A.dtype == torch.int8:
+            if scale_a is None:
+                raise ValueError("scale_a is required for already-quantised activations")
+            return gemm_int8_quantized(A, B.q, scale_a, B.scale, n=B.n, out_dtype=out_dtype)
+        if scale_a is not None:
+            raise ValueError("scale_a goes with int8 activations")
+        return linear(A, B, out_dtype=out_dtype)
+    if B.dim() != 2:
+        raise ValueError(f"B must be 2-D, got {tuple(B.shape)}")
+    if (B.shape[0] if b_layout == "kn" else B.shape[1]) != A.shape[1]:
+        raise ValueError(f"inner dimensions differ: A {tuple(A.shape)} vs B {tuple(B.shape)} ({b_layout})")
+    if A.dtype == torch.int8 and B.dtype == torch.int8:
+        if scale_a is None or scale_b is None:
+            raise ValueError("scale_a and scale_b are required for already-quantised operands")
+        qb = transpose_bytes(B) if b_layout == "kn" else B
+        return gemm_int8_quantized(A, qb, scale_a, scale_b, n=qb.shape[0], out_dtype=out_dtype)
+    if A.dtype not in _FLOAT_DTYPES or B.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"A and B must both be int8 or both be high-precision, got {A.dtype} and {B.dtype}")
+    if scale_a is not None or scale_b is not None:
+        raise ValueError("scales of high-precision operands are derived from them")
+    w = cached_pack(B, "int8", b_layout) if cache_weights else pack_weight(B, "int8", layout=b_layout)
+    return linear(A, w, out_dtype=out_dtype)
+
+
 def grouped_gemm(A: torch.Tensor, B, num_groups: Optional[int] = None, expert_offsets: Optional[torch.Tensor] = None,
                  *, format: str = "bf16", b_layout: str = "kn", out_dtype=None, cache_weights: bool = False,
                  activation: Optional[str] = None) -> torch.Tensor:
@@ -625,14 +761,14 @@ def grouped_gemm(A: torch.Tensor, B, num_groups: Optional[int] = None, expert_of
     A [sum M_g, K] with `expert_offsets` int32 [G+1] on the device -> [sum M_g, N]; groups may
     be empty and their sizes never leave the GPU.
     format "bf16" multiplies unquantised (result in A.dtype, as the Triton reference); "fp8",
-    "fp8_groupwise", "nvfp4", "mxfp4" quantise A and B on the GPU first (result fp32 unless
+    "fp8_groupwise", "int8", "nvfp4", "mxfp4" quantise A and B on the GPU first (result fp32 unless
     out_dtype says otherwise).  B may be a PackedWeight.  b_layout "kn": B [G,K,N]; "nk": [G,N,K].
     `cache_weights` as in fp8_gemm.  activation "swiglu": B is a fused gate/up projection (N = 2H, gate rows
     first, the input layout of the reference's swiglu); the result has H columns, silu(gate) * up, computed
     in the GEMM epilogue.  A PackedWeight passed as B must have been packed with `gate_up_interleave=True`.
     """
     glu = _activation_code(activation) != _lib.ACT_NONE
-    formats = {"bf16": "bf16", "fp8": "fp8", "fp8_groupwise": "fp8_block128", "nvfp4": "nvfp4", "mxfp4": "mxfp4"}
+    formats = {"bf16": "bf16", "fp8": "fp8", "fp8_groupwise": "fp8_block128", "int8": "int8", "nvfp4": "nvfp4", "mxfp4": "mxfp4"}
     if format not in formats:
         raise ValueError(f"format must be one of {sorted(formats)}, got {format!r}")
     dev = _lib.require_cuda(A, B if isinstance(B, torch.Tensor) else None, expert_offsets)

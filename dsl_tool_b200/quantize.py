@@ -71,6 +71,31 @@ def quantize_fp8(x: torch.Tensor, mode: str = "per_tensor",
     return q, s
 
 
+def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [rows, cols] (float32 / bfloat16 / float16, CUDA) -> (int8 [rows, cols], scales fp32 [rows]): one scale per row (a token,
+    or an output channel of a weight), max(amax_row / 127, 1e-12); x / scale to the nearest whole number, ties to even.  A row
+    with a NaN gets a NaN scale.  cols must be a multiple of 16, at most 32768 (a row is held in one CTA's registers)."""
+    dev = _lib.require_cuda(x)
+    x = _as_2d(x)
+    rows, cols = x.shape
+    _check_row_cols(cols)
+    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+    s = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows == 0:                       # an empty tensor has no address
+        return q, s
+    with torch.cuda.device(dev):
+        rc = _lib.lib().dsl_quant_int8(x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, s.data_ptr(), q.data_ptr(), _lib.stream_ptr())
+    _lib.check(rc, "dsl_quant_int8")
+    return q, s
+
+
+def _check_row_cols(cols: int) -> None:
+    if cols % 16 != 0:
+        raise ValueError(f"rows must be a multiple of 16 elements long, got {cols}")
+    if cols > _lib.ROW_MAX_COLS:
+        raise ValueError(f"rows must have at most {_lib.ROW_MAX_COLS} elements, got {cols}")
+
+
 def sf_bytes(rows: int, nblk: int, groups: Optional[int] = None) -> int:
     if groups is None:
         return int(_lib.lib().dsl_sf_bytes(rows, nblk))
@@ -166,9 +191,9 @@ def transpose_bytes(x: torch.Tensor) -> torch.Tensor:
 @dataclass
 class PackedWeight:
     """A weight quantised once and kept K-major ([N, K] or [G, N, K]) for repeated GEMMs."""
-    format: str                      # "fp8" | "fp8_block128" | "nvfp4" | "mxfp4" | "bf16"
-    q: torch.Tensor                  # bytes [G*N, K or K/2] (bf16: [G*N, K] bfloat16)
-    scale: Optional[torch.Tensor]    # fp8: [1]; fp8_block128: [G, N/128, K/128]; fp4: tiled scale bytes
+    format: str                      # "fp8" | "fp8_block128" | "int8" | "nvfp4" | "mxfp4" | "bf16"
+    q: torch.Tensor                  # bytes [G*N, K or K/2] (bf16: [G*N, K] bfloat16, int8: [G*N, K] int8)
+    scale: Optional[torch.Tensor]    # fp8: [1]; fp8_block128: [G, N/128, K/128]; int8: [G*N]; fp4: tiled scale bytes
     global_scale: Optional[torch.Tensor]
     groups: int
     n: int
@@ -177,7 +202,7 @@ class PackedWeight:
 
 
 _KN_K_MULTIPLE = {"fp8": 16, "fp8_block128": 16, "nvfp4": 32, "mxfp4": 32, "bf16": 8}
-_W_CODES = {"fp8": _lib.W_FP8, "fp8_block128": _lib.W_FP8_BLOCK128, "nvfp4": _lib.W_NVFP4, "mxfp4": _lib.W_MXFP4, "bf16": _lib.W_BF16}
+_W_CODES = {"fp8": _lib.W_FP8, "fp8_block128": _lib.W_FP8_BLOCK128, "nvfp4": _lib.W_NVFP4, "mxfp4": _lib.W_MXFP4, "bf16": _lib.W_BF16}   # those with a transposing quantiser
 
 
 def _pack_kn_serves(w: torch.Tensor, format: str, gate_up_interleave: bool = False) -> bool:
@@ -236,7 +261,7 @@ def _pack_weight_impl(w: torch.Tensor, format: str, layout: str = "nk",
     whole weight would.  `gate_up_interleave`: the N = 2H output rows are a fused gate/up projection
     ([gate; up], the input layout of the reference's swiglu, cuda/activations/fused_gated_activations.cu:75-90);
     they are reordered to gate_0, up_0, gate_1, up_1, ... so that `linear(..., activation="swiglu")` can fold
-    each pair in the GEMM epilogue.
+    each pair in the GEMM epilogue.  Format "int8": one scale per output channel (`quantize_int8` of the K-major rows).
     """
     dev = _lib.require_cuda(w)
     if layout not in ("nk", "kn"):
@@ -259,6 +284,11 @@ def _pack_weight_impl(w: torch.Tensor, format: str, layout: str = "nk",
     flat = w.reshape(G * N, K)
     if format == "bf16":
         return PackedWeight("bf16", flat.to(torch.bfloat16).contiguous(), None, None, G, N, K)
+    if format == "int8":
+        if global_scale is not None:
+            raise ValueError("an int8 weight has one scale per output channel: it takes no global_scale")
+        q, s = quantize_int8(flat)
+        return PackedWeight("int8", q, s, None, G, N, K)
     if format == "fp8":
         q, s = quantize_fp8(flat, "per_tensor", scale=global_scale)
         return PackedWeight("fp8", q, s, None, G, N, K)

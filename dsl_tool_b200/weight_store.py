@@ -32,9 +32,9 @@ import torch
 
 from .quantize import PackedWeight, pack_weight
 
-_DT_TO_NAME = {torch.uint8: "U8", torch.float32: "F32", torch.bfloat16: "BF16"}
+_DT_TO_NAME = {torch.uint8: "U8", torch.int8: "I8", torch.float32: "F32", torch.bfloat16: "BF16"}
 _NAME_TO_DT = {v: k for k, v in _DT_TO_NAME.items()}
-_FORMATS = ("fp8", "fp8_block128", "nvfp4", "mxfp4", "bf16")
+_FORMATS = ("fp8", "fp8_block128", "int8", "nvfp4", "mxfp4", "bf16")
 _MAX_HEADER = 1 << 20
 
 
@@ -105,7 +105,7 @@ def load_packed(path: Union[str, os.PathLike], device: Union[str, torch.device] 
         item = 2 if dt == torch.bfloat16 else torch.empty(0, dtype=dt).element_size()
         if int(np.prod(shape, dtype=np.int64)) * item != e - b:
             raise ValueError(f"{path}: tensor {name!r}: shape {shape} does not match {e - b} bytes")
-        np_dt = {torch.uint8: np.uint8, torch.float32: np.float32, torch.bfloat16: np.int16}[dt]
+        np_dt = {torch.uint8: np.uint8, torch.int8: np.int8, torch.float32: np.float32, torch.bfloat16: np.int16}[dt]
         arr = np.frombuffer(data, dtype=np_dt, count=(e - b) // item, offset=b).reshape(shape).copy()
         t = torch.from_numpy(arr)
         if dt == torch.bfloat16:

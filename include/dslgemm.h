@@ -108,6 +108,31 @@ int dsl_quant_fp4_per_token(const void* x, int dtype, long long rows, long long 
 int dsl_pack_kn(const void* w, int dtype, int groups, int K, int N, int format, int interleave, float* scale_io, int scale_given,
                 void* q_out, void* scale_out, size_t scale_bytes, void* ws, void* stream);
 
+/*
+ * int8 quantisation with one scale per row (a token of the activations, an output channel of a weight): scale_out[r] =
+ * max(amax_r / 127, 1e-12), q = x / scale to the nearest whole number (ties to even; the quotient is the IEEE fp32 one).  A row
+ * with a NaN gets a NaN scale.  x as for dsl_quant_fp8; cols % 16 == 0, cols <= DSL_ROW_MAX_COLS; q_out [rows, cols], 16-byte aligned.
+ */
+#define DSL_ROW_MAX_COLS 32768
+int dsl_quant_int8(const void* x, int dtype, long long rows, long long cols, float* scale_out, int8_t* q_out, void* stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, the result in 8 bits:
+ *   t = x + residual rounded to `dtype` (residual may be NULL: t = x);  y = (t * rsqrt(mean(t^2) + eps)) * gain in fp32;
+ *   out, scale_out = y quantised as the stand-alone quantisers would quantise it in fp32:
+ *   DSL_NORM_NONE            out [rows, cols] of `dtype`, no scale
+ *   DSL_NORM_INT8            dsl_quant_int8: int8, scale_out [rows]
+ *   DSL_NORM_FP8_GROUP_1X128 dsl_quant_fp8 in 1x128 groups: E4M3, scale_out [rows, ceil(cols/128)]
+ *   DSL_NORM_FP8_GIVEN       dsl_quant_fp8 per tensor with the given scale *scale_in (device float): E4M3
+ *   x, residual, sum_out     [rows, cols] of `dtype`, contiguous, 16-byte aligned; sum_out receives t and is required with a
+ *                            residual (it may be x or residual itself)
+ *   gain                     [cols] of `gain_dtype`
+ * cols % 16 == 0, 16 <= cols <= DSL_ROW_MAX_COLS.  A row is read once and held in one CTA's registers.
+ */
+enum { DSL_NORM_NONE = 0, DSL_NORM_INT8 = 1, DSL_NORM_FP8_GROUP_1X128 = 2, DSL_NORM_FP8_GIVEN = 3 };
+int dsl_rms_norm(const void* x, int dtype, long long rows, long long cols, const void* residual, const void* gain, int gain_dtype,
+                 float eps, int out_format, void* sum_out, void* out, float* scale_out, const float* scale_in, void* stream);
+
 /* Byte-matrix transpose [R, C] -> [C, R]: turns the reference's [K, N] weight layout
  * (cuda/gemm/fp8_gemm.cu:29-35, B[k*N+n]) into the K-major [N, K] the tensor cores read. */
 int dsl_transpose_u8(const uint8_t* in, uint8_t* out, int R, int C, void* stream);
@@ -156,7 +181,7 @@ typedef struct {
                                    bytes, ldc % 16 == 0, Nout % 16 == 0) and out_sf the scale tiles (dsl_sf_bytes /
                                    dsl_sf_bytes_grouped; zero-filled by the caller, rows of a ragged group start fresh
                                    tiles as for A).  The next GEMM can consume C / out_sf as its A / sfa directly.
-                                   Served by dsl_gemm_fp4, dsl_gemm_fp8 and dsl_gemm_bf16 (not the group-scaled FP8 GEMM). */
+                                   Served by dsl_gemm_fp4, dsl_gemm_fp8, dsl_gemm_int8 and dsl_gemm_bf16 (not the group-scaled FP8 GEMM). */
     float out_gs_host;          /* global scale of the quantised result ... */
     const float* out_gs_dev;    /* ... overridden by this device scalar when non-NULL */
     int act_scale_per_token;    /* dsl_linear with an NVFP4 weight only: quantise the activations with per-token global
@@ -180,7 +205,7 @@ int dsl_gemm_kn_served(int op, long long M, int N, int K, int groups);
  * tiles than SMs take 2 partial tiles of TOK x 128 floats per CTA (TOK = 16 or 32 tokens); other
  * problems that would leave more than half of the SMs idle take up to 8 K-slices of M x N floats.
  */
-enum { DSL_OP_GEMM_FP8 = 0, DSL_OP_GEMM_BF16 = 1, DSL_OP_GEMM_FP4_NV = 2, DSL_OP_GEMM_FP4_MX = 3, DSL_OP_GEMM_FP8_GROUPWISE = 4 };
+enum { DSL_OP_GEMM_FP8 = 0, DSL_OP_GEMM_BF16 = 1, DSL_OP_GEMM_FP4_NV = 2, DSL_OP_GEMM_FP4_MX = 3, DSL_OP_GEMM_FP8_GROUPWISE = 4, DSL_OP_GEMM_INT8 = 5 };
 size_t dsl_workspace_bytes(int op, long long M, int N, int K, int groups);
 
 /*
@@ -193,6 +218,16 @@ size_t dsl_workspace_bytes(int op, long long M, int N, int K, int groups);
  */
 int dsl_gemm_fp8(const uint8_t* A, const uint8_t* B, void* C, long long ldc, long long M_total, int N, int K,
                  const int* group_offsets, int groups, const dsl_epilogue* ep, uint32_t* status, void* stream);
+
+/*
+ * Dense / grouped INT8 GEMM: C[m,n] = (sum_k A[m,k] B[n,k]) * scale_a * scale_b * row_scale[m] * col_scale[g,n], the sum exact in
+ * int32 (also where K is cut into slices), converted to fp32 once.  With dsl_quant_int8 operands row_scale holds the tokens'
+ * scales and col_scale the channels'.  B K-major (no b_is_kn).  K % 16 == 0, K <= DSL_INT8_MAX_K (no sum can leave int32).
+ * No counterpart in the reference; conventions of dsl_gemm_fp8.
+ */
+#define DSL_INT8_MAX_K 131056
+int dsl_gemm_int8(const int8_t* A, const int8_t* B, void* C, long long ldc, long long M_total, int N, int K,
+                  const int* group_offsets, int groups, const dsl_epilogue* ep, uint32_t* status, void* stream);
 
 /*
  * Dense / grouped BF16 GEMM, fp32 accumulate (same conventions as dsl_gemm_fp8, operands bf16).
@@ -230,7 +265,8 @@ int dsl_gemm_fp4(const uint8_t* A, const uint8_t* B, const uint8_t* sfa, const u
  * entry point.  Replaces the reference's per-call sequence quantise A, quantise B, GEMM
  * (cuda/gemm/fp8_gemm.cu:180-190, cuda/gemm/fp4_gemm.cu:181-190) for a weight that was quantised once.
  *   w            the packed weight: q [groups * n, k bytes] K-major; scale = float[1] (DSL_W_FP8), 128x128 block
- *                scales [groups, ceil(n/128), k/128] (DSL_W_FP8_BLOCK128) or tiled scale bytes (FP4);
+ *                scales [groups, ceil(n/128), k/128] (DSL_W_FP8_BLOCK128), [groups * n] channel scales (DSL_W_INT8: they
+ *                and the tokens' scales take ep->col_scale and ep->row_scale, which must be NULL) or tiled scale bytes (FP4);
  *                global_scale = device float (NVFP4 only).  DSL_W_BF16: no quantisation, x must be bf16.
  *   group_offsets  int32[groups + 1] device row offsets when w->groups > 1 (ragged expert groups), else ignored
  *   act_scratch  device memory (256-byte aligned) of at least dsl_linear_scratch_bytes(format, M, k, groups) bytes
@@ -242,7 +278,7 @@ int dsl_gemm_fp4(const uint8_t* A, const uint8_t* B, const uint8_t* sfa, const u
  *                global scale (a calibrated value, device float); the quantiser then needs no amax pass and reads
  *                x once.  Otherwise the global scale is amax(x) / 2688, which costs a pass of its own.
  */
-enum { DSL_W_FP8 = 0, DSL_W_FP8_BLOCK128 = 1, DSL_W_NVFP4 = 2, DSL_W_MXFP4 = 3, DSL_W_BF16 = 4 };
+enum { DSL_W_FP8 = 0, DSL_W_FP8_BLOCK128 = 1, DSL_W_NVFP4 = 2, DSL_W_MXFP4 = 3, DSL_W_BF16 = 4, DSL_W_INT8 = 5 };
 typedef struct {
     int format;                 /* DSL_W_* */
     int groups, n, k;           /* weight is [groups, n, k] */
@@ -254,6 +290,14 @@ size_t dsl_linear_scratch_bytes(int format, long long M, int K, int groups);
 int dsl_linear(const void* x, int x_dtype, long long M, const dsl_weight* w, const int* group_offsets,
                void* act_scratch, size_t act_scratch_bytes, void* C, long long ldc, const dsl_epilogue* ep,
                uint32_t* status, void* stream);
+
+/*
+ * dsl_linear on activations that are quantised already in the weight's format (by dsl_rms_norm or a stand-alone quantiser): q
+ * [M, K] bytes with q_scale = one float (DSL_W_FP8), [M, ceil(K/128)] (DSL_W_FP8_BLOCK128) or [M] (DSL_W_INT8).  Other formats:
+ * DSL_ERR_ENUM.  ep->b_is_static as given.
+ */
+int dsl_linear_quantized(const void* q, const float* q_scale, long long M, const dsl_weight* w, const int* group_offsets, void* C,
+                         long long ldc, const dsl_epilogue* ep, uint32_t* status, void* stream);
 
 /*
  * The reference's own FP4 container (its "NVFP4" and "MXFP4" are one format, cuda/gemm/fp4_gemm.cu:30-42):
