@@ -29,6 +29,7 @@ WS_HEADER_BYTES = 64 << 10
 PER_TOKEN_MAX_COLS = 32768
 ROW_MAX_COLS = 32768
 INT8_MAX_K = 131056
+MOE_DECODE_MAX_TOKENS = 32
 
 _ERR_NAMES = {
     -1: "a required pointer is NULL",
@@ -118,6 +119,8 @@ _SIGNATURES = {
     "dsl_moe_layer_scratch_bytes": (ctypes.c_size_t, [ctypes.POINTER(Weight), ctypes.POINTER(Weight), _i, _i, _i]),
     "dsl_moe_layer": (_i, [_vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(Weight), ctypes.POINTER(Weight), _vp, _i, _f, _vp,
                            ctypes.c_size_t, _vp, _i, _vp, _vp]),
+    "dsl_moe_decode_scratch_bytes": (ctypes.c_size_t, [ctypes.POINTER(Weight), ctypes.POINTER(Weight), _i, _i, _i]),
+    "dsl_moe_decode": (_i, [_vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(Weight), ctypes.POINTER(Weight), _vp, ctypes.c_size_t, _vp, _i, _vp]),
     "dsl_moe_wire_bytes": (ctypes.c_size_t, [_i, _i]),
     "dsl_moe_reduce_pull": (_i, [ctypes.POINTER(ctypes.c_void_p), _i, _ll, _ll, _i, _i, _vp, _i, _vp]),
     "dsl_moe_pack_wire_fp4": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
@@ -157,31 +160,60 @@ def check(rc: int, what: str) -> None:
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
-    if not torch.cuda.is_available():
-        raise RuntimeError("the 'cuda' backend needs a CUDA device (sm_100a); there is no CPU fallback")
     dev = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
+            if not torch.cuda.is_available():
+                break
             raise RuntimeError("all tensors must live on a CUDA device; there is no CPU fallback")
         if dev is not None and t.device != dev:
             raise ValueError("tensors live on different devices")
         dev = t.device
+    if dev is None and not torch.cuda.is_available():      # asked only where no tensor answers it: half a microsecond
+        raise RuntimeError("the 'cuda' backend needs a CUDA device (sm_100a); there is no CPU fallback")
     return dev
 
 
-def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+# The handle alone, without the Stream object around it (0.2 us instead of 3.2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_ptr(index: Optional[int] = None) -> int:
+    """Handle of the current stream of device `index` (default: the current device)."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(index).cuda_stream
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+class on_device:
+    """`with on_device(dev):` - torch.cuda.device(dev) for the usual case that it is current already, at a tenth of the host time."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, dev: torch.device) -> None:
+        self.index = dev.index
+
+    def __enter__(self) -> None:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
 def dtype_code(dt: torch.dtype) -> int:
     try:
-        return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}[dt]
+        return _DTYPE_CODES[dt]
     except KeyError:
         raise TypeError(f"unsupported input dtype {dt}; use float32, bfloat16 or float16") from None
 

@@ -11,16 +11,18 @@
 //
 // Bound by memory: x, r and w are read once, t, q and s written once (8192 x 8192 bf16 with residual: 403 MB).  One CTA takes a
 // row and keeps it in registers, 16 consecutive elements a thread, so the three looks at it (sum of squares, maximum, conversion)
-// cost one trip to memory; a CTA has as many threads as the row has 16-element pieces (a row of 4096: 256 threads, eight rows an
-// SM in flight), and rows beyond 1024 pieces give every thread two.  The two sums over a row are a shuffle tree and one meeting
-// in shared memory each; other CTAs of the SM cover it.
+// cost one trip to memory; a CTA has as many threads as the row has 16-element pieces (a row of 4096: 256 threads), and rows beyond
+// 1024 pieces give every thread two.  The reductions over a row are a shuffle tree and one meeting in shared memory each.
 //
 // A NaN anywhere in a row makes an int8 row's scale NaN (an integer cannot carry it): the maximum is taken over the bit patterns
 // of |y|, where every NaN is above infinity.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "dslgemm.h"
+#include "gemm.cuh"
 #include "norm.cuh"
 #include "ptx.cuh"
 #include "quant_math.cuh"
@@ -39,6 +41,7 @@ struct RowArgs {
     float* scale_out;          // int8 [rows]; FP8 1x128 [rows, ceil(cols / 128)]
     const float* scale_in;     // FP8 given: one float
     float eps;
+    long long rows;
     int cols;
     bool wide;                 // rows of x, residual and sum start on 32-byte boundaries
 };
@@ -127,127 +130,185 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
     return __reduce_max_sync(0xFFFFFFFFu, lane < warps ? slots[lane] : 0u);
 }
 
-// PIECES: 16-element pieces a thread holds; piece p of thread i starts at (p * blockDim.x + i) * 16.
-template <typename T, int OUT, bool NORM, int PIECES>
-__global__ void __launch_bounds__(1024) row_kernel(const RowArgs a) {
-    __shared__ float s_sum[32];
-    __shared__ uint32_t s_max[32];
+// 16 elements as they lie in memory: 8 words of a 16-bit type, 16 of fp32.
+template <typename T>
+struct Raw16 {
+    static constexpr int WORDS = static_cast<int>(sizeof(T)) * 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* p, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 8) {
+                uint32_t t[8];
+                ldg256(reinterpret_cast<const uint32_t*>(p) + i, t);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[i + j] = t[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 t = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i));
+                w[i] = t.x; w[i + 1] = t.y; w[i + 2] = t.z; w[i + 3] = t.w;
+            }
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        if (dsl_is_half<T>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i / 2]));
+            return i & 1 ? f.y : f.x;
+        }
+        return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    }
+};
+
+// PIECES: 16-element pieces a thread holds; piece p of thread i starts at (p * blockDim.x + i) * 16.  A CTA walks rows blockIdx.x,
+// + gridDim.x, ...; the next row's loads are issued before this row's meetings (where registers allow it: one piece a thread), so
+// that memory is busy while the CTA waits for itself: 8192 x 8192 bf16, residual, FP8 groups: one row a CTA 105 us, so NORM_US us.
+template <typename T, int OUT, bool NORM, int PIECES, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS, sizeof(T) == 2 ? 1024 / MAX_THREADS : 1) row_kernel(const RowArgs a) {
+    constexpr bool AHEAD = PIECES == 1 && (sizeof(T) == 2 || MAX_THREADS <= 512);
+    __shared__ float s_sum[2][32];
+    __shared__ uint32_t s_max[2][32];
     // Launched as a dependent: placed while the kernel before it drains.  What follows may do the same once that one is complete.
     griddep_wait();
     griddep_launch_dependents();
-    const size_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(a.x) + row * a.cols;
-    float v[PIECES][16];
-#pragma unroll
-    for (int p = 0; p < PIECES; ++p) {
+    const bool with_residual = NORM && a.residual != nullptr;
+    Raw16<T> rx[PIECES], rr[PIECES];
+    auto fetch = [&](long long row, int p) {
         const int at = (p * blockDim.x + threadIdx.x) * 16;
         if (at < a.cols) {
-            load16w<T>(x + at, v[p], a.wide);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[p][i] = 0.f;
+            rx[p].load(static_cast<const T*>(a.x) + row * a.cols + at, a.wide);
+            if (with_residual) rr[p].load(static_cast<const T*>(a.residual) + row * a.cols + at, a.wide);
         }
-    }
-    if (NORM) {
-        float squares = 0.f;
-        if (a.residual != nullptr) {
-            const T* r = static_cast<const T*>(a.residual) + row * a.cols;
-            T* t = static_cast<T*>(a.sum_out) + row * a.cols;
+    };
+    if (AHEAD) fetch(blockIdx.x, 0);
+    int parity = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        float v[PIECES][16];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            if (!AHEAD) fetch(row, p);
+            const int at = (p * blockDim.x + threadIdx.x) * 16;
+            if (at < a.cols) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[p][i] = rx[p].at(i);
+                if (with_residual) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[p][i] = round_to<T>(__fadd_rn(v[p][i], rr[p].at(i)));
+                    store16<T>(static_cast<T*>(a.sum_out) + row * a.cols + at, v[p]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[p][i] = 0.f;
+            }
+        }
+        if (AHEAD && row + gridDim.x < a.rows) fetch(row + gridDim.x, 0);
+        if (NORM) {
+            float squares = 0.f;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) squares = fmaf(v[p][i], v[p][i], squares);
+            squares = block_sum(squares, s_sum[parity]);
+            const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares, static_cast<float>(a.cols)), a.eps));
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
                 const int at = (p * blockDim.x + threadIdx.x) * 16;
-                if (at >= a.cols) break;
-                float b[16];
-                load16w<T>(r + at, b, a.wide);
+                if (at < a.cols) {
+                    float w[16];
+                    load_gain(a.gain, a.gain_dtype, at, w);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[p][i] = round_to<T>(__fadd_rn(v[p][i], b[i]));
-                store16<T>(t + at, v[p]);
+                    for (int i = 0; i < 16; ++i) v[p][i] = __fmul_rn(__fmul_rn(v[p][i], inv), w[i]);
+                }
             }
         }
+        uint8_t* q = static_cast<uint8_t*>(a.out) + row * a.cols;
+        float s = 0.f;
+        if (OUT == ROW_INT8) {
+            uint32_t m = 0u;
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
+            for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) squares = fmaf(v[p][i], v[p][i], squares);
-        squares = block_sum(squares, s_sum);
-        const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares, static_cast<float>(a.cols)), a.eps));
+                for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
+            s = int8_scale_from_amax(__uint_as_float(block_max(m, s_max[parity])));
+            if (threadIdx.x == 0) a.scale_out[row] = s;
+        }
+        if (OUT == ROW_FP8_GIVEN) s = *a.scale_in;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int at = (p * blockDim.x + threadIdx.x) * 16;
-            if (at >= a.cols) break;
-            float w[16];
-            load_gain(a.gain, a.gain_dtype, at, w);
+            if (OUT == ROW_FP8_GROUP) {      // eight neighbouring threads hold a group; threads past the row's end hold zeros
+                float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[p][i] = __fmul_rn(__fmul_rn(v[p][i], inv), w[i]);
-        }
-    }
-    uint8_t* q = static_cast<uint8_t*>(a.out) + row * a.cols;
-    float s = 0.f;
-    if (OUT == ROW_INT8) {
-        uint32_t m = 0u;
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[p][i]));
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
-        s = int8_scale_from_amax(__uint_as_float(block_max(m, s_max)));
-        if (threadIdx.x == 0) a.scale_out[row] = s;
-    }
-    if (OUT == ROW_FP8_GIVEN) s = *a.scale_in;
-#pragma unroll
-    for (int p = 0; p < PIECES; ++p) {
-        const int at = (p * blockDim.x + threadIdx.x) * 16;
-        if (OUT == ROW_FP8_GROUP) {      // eight neighbouring threads hold a group; threads past the row's end hold zeros
-            float m = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[p][i]));
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            s = fp8_scale_from_amax(m);
-            if (at < a.cols && (threadIdx.x & 7) == 0) a.scale_out[row * ((a.cols + 127) / 128) + at / 128] = s;
-        }
-        if (at < a.cols) {
-            if (OUT == ROW_NONE) store16<T>(static_cast<T*>(a.out) + row * a.cols + at, v[p]);
-            else if (OUT == ROW_INT8) *reinterpret_cast<uint4*>(q + at) = quant16_int8(v[p], s);
-            else *reinterpret_cast<uint4*>(q + at) = quant16_e4m3<OUT == ROW_FP8_GIVEN>(v[p], s);
+                for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+                s = fp8_scale_from_amax(m);
+                if (at < a.cols && (threadIdx.x & 7) == 0) a.scale_out[row * ((a.cols + 127) / 128) + at / 128] = s;
+            }
+            if (at < a.cols) {
+                if (OUT == ROW_NONE) store16<T>(static_cast<T*>(a.out) + row * a.cols + at, v[p]);
+                else if (OUT == ROW_INT8) *reinterpret_cast<uint4*>(q + at) = quant16_int8(v[p], s);
+                else *reinterpret_cast<uint4*>(q + at) = quant16_e4m3<OUT == ROW_FP8_GIVEN>(v[p], s);
+            }
         }
     }
 }
 
-template <typename T, int OUT, bool NORM>
-static cudaError_t launch_row(const RowArgs& a, long long rows, cudaStream_t st) {
-    const int pieces = a.cols / 16;
+template <typename T, int OUT, bool NORM, int PIECES, int MAX_THREADS>
+static cudaError_t launch_threads(const RowArgs& a, int threads, cudaStream_t st) {
+    // CTAs an SM holds, by warps a CTA, asked once per device
+    static std::atomic<int> resident_of[DSL_MAX_DEVICES][33];
+    const int dev = current_device_slot();
+    if (dev < 0) return cudaErrorInvalidDevice;
+    int resident = resident_of[dev][threads / 32].load(std::memory_order_relaxed);
+    if (resident == 0) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_kernel<T, OUT, NORM, PIECES, MAX_THREADS>, threads, 0);
+        if (e != cudaSuccess) return e;
+        if (resident < 1) resident = 1;
+        resident_of[dev][threads / 32].store(resident, std::memory_order_relaxed);
+    }
+    const long long ctas = static_cast<long long>(sm_count()) * resident;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows));
+    cfg.gridDim = dim3(static_cast<unsigned>(a.rows < ctas ? a.rows : ctas));
+    cfg.blockDim = dim3(threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (pieces <= 1024) {
-        cfg.blockDim = dim3((pieces + 31) / 32 * 32);
-        return cudaLaunchKernelEx(&cfg, row_kernel<T, OUT, NORM, 1>, a);
-    }
-    cfg.blockDim = dim3(((pieces + 1) / 2 + 31) / 32 * 32);
-    return cudaLaunchKernelEx(&cfg, row_kernel<T, OUT, NORM, 2>, a);
+    return cudaLaunchKernelEx(&cfg, row_kernel<T, OUT, NORM, PIECES, MAX_THREADS>, a);
+}
+
+template <typename T, int OUT, bool NORM>
+static cudaError_t launch_row(const RowArgs& a, cudaStream_t st) {
+    const int pieces = a.cols / 16;
+    const int threads = (pieces + 31) / 32 * 32;
+    if (threads <= 512) return launch_threads<T, OUT, NORM, 1, 512>(a, threads, st);
+    if (threads <= 1024) return launch_threads<T, OUT, NORM, 1, 1024>(a, threads, st);
+    return launch_threads<T, OUT, NORM, 2, 1024>(a, ((pieces + 1) / 2 + 31) / 32 * 32, st);
 }
 
 template <typename T>
-static cudaError_t launch_type(const RowArgs& a, int format, bool norm, long long rows, cudaStream_t st) {
-    if (!norm) return launch_row<T, ROW_INT8, false>(a, rows, st);
+static cudaError_t launch_type(const RowArgs& a, int format, bool norm, cudaStream_t st) {
+    if (!norm) return launch_row<T, ROW_INT8, false>(a, st);
     switch (format) {
-        case ROW_INT8: return launch_row<T, ROW_INT8, true>(a, rows, st);
-        case ROW_FP8_GROUP: return launch_row<T, ROW_FP8_GROUP, true>(a, rows, st);
-        case ROW_FP8_GIVEN: return launch_row<T, ROW_FP8_GIVEN, true>(a, rows, st);
-        default: return launch_row<T, ROW_NONE, true>(a, rows, st);
+        case ROW_INT8: return launch_row<T, ROW_INT8, true>(a, st);
+        case ROW_FP8_GROUP: return launch_row<T, ROW_FP8_GROUP, true>(a, st);
+        case ROW_FP8_GIVEN: return launch_row<T, ROW_FP8_GIVEN, true>(a, st);
+        default: return launch_row<T, ROW_NONE, true>(a, st);
     }
 }
 
 static cudaError_t launch_dtype(RowArgs& a, int dtype, int format, bool norm, long long rows, cudaStream_t st) {
+    a.rows = rows;
     const uintptr_t all = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual);
     a.wide = (all & 31u) == 0;           // a row is a multiple of 16 elements, i.e. of 32 bytes
-    if (dtype == DSL_F32) return launch_type<float>(a, format, norm, rows, st);
-    if (dtype == DSL_BF16) return launch_type<__nv_bfloat16>(a, format, norm, rows, st);
-    return launch_type<__half>(a, format, norm, rows, st);
+    if (dtype == DSL_F32) return launch_type<float>(a, format, norm, st);
+    if (dtype == DSL_BF16) return launch_type<__nv_bfloat16>(a, format, norm, st);
+    return launch_type<__half>(a, format, norm, st);
 }
 
 cudaError_t launch_quant_int8(const void* x, int dtype, long long rows, int cols, float* scale_out, int8_t* q, cudaStream_t st) {

@@ -120,8 +120,8 @@ def _run(dev, ep: "_lib.Epilogue", problem: tuple, launch) -> int:
     """One GEMM entry point: `launch(status, stream)` -> return code.  `problem` = (DSL_OP_* code, M, N, K, groups): the
     scratch that the kernels can use for it (dsl_workspace_bytes) is the current stream's, and its lock is held over
     the call, whose launches hand sums to one another through it."""
-    with torch.cuda.device(dev):
-        status, stream = _lib.status_word(dev).data_ptr(), _lib.stream_ptr()
+    with _lib.on_device(dev):
+        status, stream = _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev.index)
         need = int(_lib.lib().dsl_workspace_bytes(*problem))
         if need <= 0:
             return launch(status, stream)
@@ -352,7 +352,7 @@ def _new_weight_desc(w: PackedWeight) -> "_lib.Weight":
 def _weight_desc(w: PackedWeight) -> "_lib.Weight":
     """The weight's dsl_weight struct, built once and kept on the PackedWeight (rebuilt if its tensors were swapped)."""
     d = getattr(w, "_cdesc", None)
-    if d is None or d.q != w.q.data_ptr():
+    if d is None or d.q != w.q.data_ptr() or d.scale != _lib.ptr(w.scale) or d.global_scale != _lib.ptr(w.global_scale):
         d = _new_weight_desc(w)
         w._cdesc = d
         w._scratch_need = {}
@@ -411,7 +411,7 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
             need = int(lib.dsl_linear_scratch_bytes(desc.format, M, w.k, groups))
             if len(w._scratch_need) < 64:
                 w._scratch_need[M] = need
-        stream = torch.cuda.current_stream(dev).cuda_stream
+        stream = _lib.stream_ptr(dev.index)
         scratch, capturing = _lib.act_arena(dev, stream), torch.cuda.is_current_stream_capturing()
         with scratch.lock:
             buf = scratch.get(dev, need, capturing) if need else None

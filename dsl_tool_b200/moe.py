@@ -31,7 +31,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .gemm_kernels import _BYTE_DTYPES, _new_weight_desc, gemm_fp4_quantized, gemm_fp8_groupwise_quantized, gemm_fp8_quantized, linear
+from .gemm_kernels import _BYTE_DTYPES, _FLOAT_DTYPES, _new_weight_desc, _weight_desc, gemm_fp4_quantized, gemm_fp8_groupwise_quantized, gemm_fp8_quantized, linear
 from .quantize import PackedWeight, pack_weight, quantize_fp4, quantize_fp8
 from .sharding import arrival_expert_ids, exchange_rows, expert_ranges, return_rows
 
@@ -202,6 +202,9 @@ def _as_packed(w: PackedWeight, device: torch.device) -> bool:
         return False
     if fmt == "bf16":
         return q.dtype is torch.bfloat16 and q.shape == (rows, k)
+    if fmt == "int8":
+        return (q.dtype is torch.int8 and q.shape == (rows, k) and scale is not None and scale.dtype is torch.float32
+                and scale.numel() == rows and scale.device == device and scale.is_contiguous())
     if q.dtype not in _BYTE_DTYPES or scale is None or scale.device != device or not scale.is_contiguous():
         return False
     tiles = w.groups * ((w.n + 127) // 128)
@@ -260,6 +263,61 @@ def _whole_layer(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, r
         if prev != dev.index:
             torch.cuda.set_device(prev)
     _lib.check(rc, "dsl_moe_layer")
+    return out
+
+
+def moe_decode(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, *, renormalize: bool = True,
+               out_dtype=torch.float32) -> torch.Tensor:
+    """The layer for at most 32 tokens on a GPU that holds every expert, in two kernels: x [tokens, K] (float32, bfloat16 or
+    float16), logits [tokens, experts] (float32 or bfloat16) -> [tokens, D] (float32 or bfloat16).
+
+    Where `moe_forward` quantises the activations for the grouped GEMMs, here they stay as they are (weight-only quantisation):
+    with a row or two for each chosen expert the layer is the reading of those experts' weights.  Routing is `route`'s: softmax,
+    the k largest, ties to the lower index; an expert whose logit is minus infinity or NaN is never chosen, and a token left
+    without any gets zeros.  Weights of every packed format ("fp8", "fp8_block128", "int8", "nvfp4", "mxfp4", "bf16") as
+    `MoEWeights.pack` makes them.  Sums are fp32; a float32 x and the hidden activation are rounded to 11 bits (16 with bf16
+    weights).  The result does not depend on how many tokens share the call.  More tokens: `moe_forward`."""
+    gu, dn = w.gate_up, w.down
+    dev = _lib.require_cuda(x, logits, gu.q, dn.q)
+    if x.dim() != 2 or x.shape[1] != gu.k:
+        raise ValueError(f"x must be [tokens, {gu.k}], got {tuple(x.shape)}")
+    T = x.shape[0]
+    if x.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.shape != (T, w.experts):
+        raise ValueError(f"logits must be [{T}, {w.experts}], got {tuple(logits.shape)}")
+    if T > _lib.MOE_DECODE_MAX_TOKENS:
+        raise ValueError(f"at most {_lib.MOE_DECODE_MAX_TOKENS} tokens, got {T}: moe_forward takes any number")
+    if not 1 <= k <= min(32, w.experts):
+        raise ValueError(f"k must lie between 1 and {min(32, w.experts)}, got {k}")
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
+    if w.first != 0 or w.last != w.experts or gu.groups != w.experts or dn.groups != w.experts:
+        raise ValueError(f"moe_decode needs all {w.experts} experts on this GPU, the weights hold {w.first} .. {w.last}")
+    if gu.format != dn.format or gu.n != 2 * dn.k or not gu.gate_up_interleaved:
+        raise ValueError(f"gate/up ({gu.format} [{gu.n}, {gu.k}]) must be packed with gate_up_interleave=True and match down "
+                         f"({dn.format} [{dn.n}, {dn.k}])")
+    if not (_as_packed(gu, dev) and _as_packed(dn, dev)):
+        raise ValueError("the weights' tensors are not as pack_weight lays them out")
+    out = torch.empty((T, dn.n), dtype=out_dtype, device=dev)
+    if T == 0:
+        return out
+    x, logits = x.contiguous(), logits.contiguous()
+    lib, du, dd, code = _lib.lib(), ctypes.byref(_weight_desc(gu)), ctypes.byref(_weight_desc(dn)), _lib.dtype_code(x.dtype)
+    with _lib.on_device(dev):
+        need = int(lib.dsl_moe_decode_scratch_bytes(du, dd, T, k, code))
+        if need == 0:
+            raise ValueError(f"moe_decode does not take rows of {gu.k} and {dn.k} elements of {gu.format}: multiples of 32 (FP4), 128 "
+                             "(128x128 FP8), 16 (FP8, int8) or 8 (bf16), and a row has to fit a CTA's shared memory")
+        stream = _lib.stream_ptr(dev.index)
+        scratch, capturing = _lib.act_arena(dev, stream), torch.cuda.is_current_stream_capturing()
+        with scratch.lock:
+            buf = scratch.get(dev, need, capturing)
+            rc = lib.dsl_moe_decode(x.data_ptr(), code, logits.data_ptr(), _lib.dtype_code(logits.dtype), T, k, 1 if renormalize else 0,
+                                    du, dd, buf.data_ptr(), need, out.data_ptr(), _lib.dtype_code(out_dtype), stream)
+    _lib.check(rc, "dsl_moe_decode")
     return out
 
 

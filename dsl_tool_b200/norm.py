@@ -47,12 +47,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
         raise ValueError(f"weight must be [{cols}], got {tuple(weight.shape)}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must have the shape and type of x, got {tuple(residual.shape)} {residual.dtype}")
-    x2 = _as_2d(x)
+    x2 = x if x.dim() == 2 and x.is_contiguous() else _as_2d(x)
     rows = x2.shape[0]
     weight = weight.contiguous()
     r2 = total = s = s_in = None
     if residual is not None:
-        r2 = _as_2d(residual)
+        r2 = residual if residual.dim() == 2 and residual.is_contiguous() else _as_2d(residual)
         total = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if format is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
@@ -67,9 +67,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
                     else torch.full((1,), float(scale), dtype=torch.float32, device=dev))
     if rows == 0:                       # an empty tensor has no address
         return out, s, total
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.lib().dsl_rms_norm(x2.data_ptr(), _lib.dtype_code(x2.dtype), rows, cols, _lib.ptr(r2), weight.data_ptr(),
                                      _lib.dtype_code(weight.dtype), eps, _FORMATS[format], _lib.ptr(total), out.data_ptr(), _lib.ptr(s),
-                                     _lib.ptr(s_in), _lib.stream_ptr())
+                                     _lib.ptr(s_in), _lib.stream_ptr(dev.index))
     _lib.check(rc, "dsl_rms_norm")
     return out, s, total

@@ -83,8 +83,9 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     s = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows == 0:                       # an empty tensor has no address
         return q, s
-    with torch.cuda.device(dev):
-        rc = _lib.lib().dsl_quant_int8(x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, s.data_ptr(), q.data_ptr(), _lib.stream_ptr())
+    with _lib.on_device(dev):
+        rc = _lib.lib().dsl_quant_int8(x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, s.data_ptr(), q.data_ptr(),
+                                       _lib.stream_ptr(dev.index))
     _lib.check(rc, "dsl_quant_int8")
     return q, s
 

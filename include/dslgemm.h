@@ -366,6 +366,21 @@ int dsl_moe_layer(const void* x, int x_dtype, const void* logits, int logits_dty
                   const dsl_weight* gate_up, const dsl_weight* down, const float* act_gs_dev, int fused_hidden,
                   float hidden_gs, void* scratch, size_t scratch_bytes, void* out, int out_dtype, uint32_t* status,
                   void* stream);
+/*
+ * The layer for a few tokens in two kernels, activations unquantised: route, gate/up with SwiGLU, down, combine, each chosen
+ * expert's weights read once.  Weights as for dsl_moe_layer, DSL_W_INT8 too; x in any of the three types.  Rounding: weights and
+ * 16-bit x exact, an fp32 x and the hidden activation to 11 bits (16 with BF16 weights), sums in fp32.  An expert whose logit is
+ * minus infinity or NaN is never chosen; a token without any gets zeros.  At most DSL_MOE_DECODE_MAX_TOKENS tokens, k <= 32; K
+ * and H multiples of 32 (FP4), 128 (128x128 FP8), 16 (FP8, INT8) or 8 (BF16), at most 2^20, and short enough that one row fits a
+ * CTA's shared memory beside the routing tables (some 36000 elements at the least); else DSL_ERR_TOO_LARGE.
+ *   scratch     dsl_moe_decode_scratch_bytes bytes, 256-byte aligned, consumed within the call: calls issued in order on one
+ *               stream may share it, calls that can overlap may not.  0 bytes: a problem that the call does not take
+ */
+#define DSL_MOE_DECODE_MAX_TOKENS 32
+size_t dsl_moe_decode_scratch_bytes(const dsl_weight* gate_up, const dsl_weight* down, int tokens, int k, int x_dtype);
+int dsl_moe_decode(const void* x, int x_dtype, const void* logits, int logits_dtype, int tokens, int k, int renorm,
+                   const dsl_weight* gate_up, const dsl_weight* down, void* scratch, size_t scratch_bytes, void* out, int out_dtype,
+                   void* stream);
 size_t dsl_moe_wire_bytes(int K, int format);
 /*
  * Sum of the ranks' partial results over peer memory (expert-parallel layer whose ranks keep their own token rows; no

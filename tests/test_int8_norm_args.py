@@ -104,3 +104,38 @@ def test_registered_with_the_dispatcher():
     from dsl_tool_b200.dispatcher import KernelDispatcher
     info = KernelDispatcher().kernel_info("gemm.int8_gemm", "cuda")
     assert {"A", "B", "scale_a", "scale_b", "b_layout", "out_dtype"} <= set(info["input_schema"])
+
+
+def test_moe_decode_arguments(cdll):
+    keep, p = _buffer()
+
+    def weight(fmt, n, k, groups=4, q=p, scale=p, gs=p):
+        w = _lib.Weight()
+        w.format, w.groups, w.n, w.k, w.q, w.scale, w.global_scale = fmt, groups, n, k, q, scale, gs
+        return w
+
+    def need(gu, dn, tokens=2, k=2, x_dtype=_lib.BF16):
+        return cdll.dsl_moe_decode_scratch_bytes(ctypes.byref(gu), ctypes.byref(dn), tokens, k, x_dtype)
+
+    def call(gu, dn, tokens=2, k=2, x=p, x_dtype=_lib.BF16, logits=p, l_dtype=0, scratch=p, nbytes=1 << 30, out=p, o_dtype=0):
+        return cdll.dsl_moe_decode(x, x_dtype, logits, l_dtype, tokens, k, 1, ctypes.byref(gu), ctypes.byref(dn), scratch, nbytes, out, o_dtype, None)
+    for fmt, m in ((_lib.W_FP8, 16), (_lib.W_FP8_BLOCK128, 128), (_lib.W_INT8, 16), (_lib.W_NVFP4, 32), (_lib.W_MXFP4, 32), (_lib.W_BF16, 8)):
+        gu, dn = weight(fmt, 4 * m, 3 * m), weight(fmt, 40, 2 * m)
+        assert need(gu, dn) >= 4 * 4 * (2 * m + 40)
+        assert need(weight(fmt, 4 * m, 3 * m + m // 2), dn) == 0                # K not a multiple
+        assert need(gu, weight(fmt, 40, m)) == 0                                # H does not match
+        assert need(gu, dn, tokens=33) == 0 and need(gu, dn, k=5) == 0 and need(gu, dn, k=0) == 0 and need(gu, dn, x_dtype=3) == 0
+        assert call(gu, dn, x=None) == -1 and call(gu, dn, logits=None) == -1 and call(gu, dn, out=None) == -1
+        assert call(gu, dn, scratch=None) == -1 and call(weight(fmt, 4 * m, 3 * m, q=None), dn) == -1
+        assert call(gu, dn, x=p + 8) == -3 and call(gu, dn, scratch=p + 16) == -3
+        assert call(gu, dn, l_dtype=2) == -4 and call(gu, dn, o_dtype=2) == -4
+        assert call(gu, dn, nbytes=need(gu, dn) - 1) == -6 and call(gu, dn, tokens=33) == -6
+        assert call(gu, dn, tokens=0) == 0
+    gu, dn = weight(_lib.W_NVFP4, 128, 64, gs=None), weight(_lib.W_NVFP4, 40, 64)
+    assert call(gu, dn) == -1
+    assert need(weight(_lib.W_FP8, 64, 64), weight(_lib.W_INT8, 40, 32)) == 0   # two formats
+    assert need(weight(6, 64, 64), weight(6, 40, 32)) == 0
+    assert need(weight(_lib.W_BF16, 64, 65536), weight(_lib.W_BF16, 40, 32), x_dtype=_lib.F32) == 0      # a row that does not fit
+    for K in (36000, 32768):
+        assert need(weight(_lib.W_BF16, 64, K), weight(_lib.W_BF16, 40, 32), tokens=1, x_dtype=_lib.F32) > 0
+    del keep
