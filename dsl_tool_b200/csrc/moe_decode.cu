@@ -6,18 +6,22 @@
 // With one or two rows for each chosen expert the layer is the reading of those experts' weights, so everything is arranged round
 // that stream and the activations stay unquantised (nothing would be gained from fewer bits of them).
 //
-//   * Work is the list of (expert, tile of 16 weight rows) pairs, expert by expert; CTA b of the grid (one an SM) takes the b-th
-//     equal share.  The list follows from the logits; every CTA makes it for itself in shared memory (a few hundred
-//     nanoseconds), so nothing has to be launched, sorted or copied before.
-//   * A CTA keeps the rows of x (or h) that its current expert multiplies in shared memory, as 16-bit values in the order in which
-//     the tensor core's B fragments want them.  Weights go from global memory straight into registers (16 warps x 8 loads of 16
-//     bytes a lane in flight: 64 KB an SM), are widened there to f16 or bf16, exactly, and meet the rows in mma.sync m16n8k16 with
-//     fp32 sums.  The order of K inside a 16-row x 64-byte chunk is free as long as both sides agree: lane (g, t) of a warp holds
-//     16 consecutive bytes of weight rows g and g + 8, every load of a warp covers whole 64-byte pieces, and no weight passes
-//     through shared memory.  (tcgen05 would want the widened weight written to shared memory first, for tiles of which at most
-//     one column in eight is used; the warp-wide instruction runs far below its rate here.)
-//   * K of a tile is cut over `split` warps when there are few tiles; their sums meet in shared memory, in order.
-//   * Down's results go to scratch by (token, slot); the CTA that delivers a tile's last one adds the slots and writes the output.
+//   * Work is the list of (expert, unit of 16 weight rows) pairs, expert by expert; CTA b of the grid (one an SM) takes the b-th
+//     equal share.  The list follows from the logits; every CTA makes it for itself in shared memory, so nothing has to be launched,
+//     sorted or copied before.
+//   * Two units make a tile of 32 rows, {q * 8 + g + 32 j : g < 8, j < 4} of a block of 128: the rows whose FP4 scale bytes lie
+//     side by side, so that one 16-byte load brings a lane the scales of all its rows.  A step is 64 bytes of a tile's rows.
+//   * A CTA's steps, tile after tile, are dealt to its 16 warps in equal runs.  A tile that lies inside a run is finished by its
+//     warp; the pieces of the others meet in shared memory after the last step and are added in order.
+//   * The rows of x (or h) that the current expert multiplies are kept in shared memory, as 16-bit values in the order in which the
+//     tensor core's B fragments want them.  Weights go from global memory straight into registers (two or three steps of four
+//     16-byte loads a lane in flight while another is multiplied: 64 or 96 KB an SM), are widened there to f16 or bf16, exactly, and meet the
+//     rows in mma.sync m16n8k16 with fp32 sums.  The order of K inside a step is free as long as both sides agree: lane (g, t) of
+//     a warp holds 16 consecutive bytes of its four rows, every load covers whole 64-byte pieces, and no weight passes through
+//     shared memory.  (tcgen05 would want the widened weight written to shared memory first, for tiles of which at most one column
+//     in eight is used.  The widening - two instructions for two FP4 weights - and not the products' rate is what the FP4 formats
+//     are bound by: an SM widens 64 pairs a clock, and HBM brings 23.)
+//   * Down's results go to scratch by (token, slot); the CTA that delivers a unit's last one adds the slots and writes the output.
 //     Which CTA that is changes nothing: it adds in slot order.
 //
 // Rounding.  Weights are exact in the 16-bit type: E4M3, e2m1 x UE4M3 and int8 in f16, bf16 in bf16; MXFP4's power-of-two scales
@@ -30,6 +34,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
+#include <stdlib.h>
 
 #include <atomic>
 
@@ -42,9 +47,9 @@ namespace md {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
-constexpr int STEP = 256;                // bytes of a weight row that a warp takes at once: 4 chunks of 64
-constexpr int MAX_ENTRIES = DSL_MOE_DECODE_MAX_TOKENS * 32;
-constexpr int RED_PITCH = 20;            // floats between two columns of a warp's 16-row sums: no bank conflicts on either side
+constexpr int SUM_FLOATS = 8 * 36;       // a tile's sums: eight columns of 32 rows, 36 apart (no bank conflicts)
+constexpr int STEP = 64;                 // bytes of a weight row that a warp takes at once
+constexpr int MIN_STEPS = 4;             // of a tile (short rows: steps without bytes)
 
 enum { F8 = 0, F8G = 1, I8 = 2, NV = 3, MX = 4, BF = 5 };
 
@@ -53,6 +58,9 @@ struct Fmt {
     static constexpr int ELEMS = FMT == NV || FMT == MX ? 32 : (FMT == BF ? 8 : 16);     // in 16 bytes
     static constexpr bool BF16 = FMT == BF;                                              // type of the products
     static constexpr int PARTS = FMT == BF ? 2 : 1;                                      // 16-bit terms of an activation, at most
+    static constexpr bool FP4 = FMT == NV || FMT == MX;
+    static constexpr int AHEAD = FP4 ? 3 : 4;            // steps that a lane has registers for: all but one in flight
+    static constexpr int ROWS = FMT == MX ? 4 : 8;       // activation rows that a CTA multiplies at a time, at most
 };
 
 struct Args {
@@ -63,131 +71,162 @@ struct Args {
     const uint8_t* w;            // [experts, n, row_bytes]
     const uint8_t* scale;        // as the packed weight has it
     const float* global_scale;
-    int n, kdim, row_bytes, katoms, tiles, steps, split;
+    int n, kdim, row_bytes, katoms;
+    int units;                   // of 16 rows: 8 for every 128, the last ones possibly without rows
+    int entry_cost;              // what starting on an expert costs a CTA, in units
+    int steps;                   // of a tile
+    unsigned div_span, div_steps, div_grid, div_k;      // 2^32 / (units + entry_cost), / steps, / CTAs, / k: see quotient()
     int block_rows;              // rows of one expert that a CTA holds at a time
     int parts;                   // 16-bit terms an activation (2 only with bf16 products)
     float* h;                    // up: [entries, n / 2]
     float* y;                    // down: [entries, n]
-    int* arrived;                // down: one counter a tile, zeroed by up
+    int* arrived;                // down: one counter a unit, zeroed by up
     int arrived_count;
     void* out;                   // down: [tokens, n]
     int out_dtype;
 };
+
+// n / d for n < 2^31, with m = floor((2^32 - 1) / d): the estimate is at most one too small.
+__device__ __forceinline__ int quotient(int n, int d, unsigned m) {
+    const int q = static_cast<int>(__umulhi(static_cast<unsigned>(n), m));
+    return n - q * d >= d ? q + 1 : q;
+}
 
 // ---- routing -------------------------------------------------------------------------------------------------------------------
 // Shared-memory tables of the list of work: entry = token * k + slot.
 struct Plan {
     int* ids;          // [entries] expert, or -1
     float* weights;    // [entries]
-    int* order;        // entries sorted by expert, stable
+    int* order;        // entries sorted by expert, an expert's by token
     int* seg_expert;   // [segments]: an expert with at most block_rows of its rows
     int* seg_first;    //             first place in `order`
     int* seg_rows;
-    int* count;        // [experts]
+    uint32_t* tokens;  // [experts] who chose it, a bit each
+    int* base;         // [experts] its first place in `order`
     int segments;
 };
 
-// Softmax over the experts and the k largest, ties to the lower index; the arithmetic of moe_route_kernel (moe.cu).  A logit of
-// minus infinity or NaN is never chosen: an entry without an expert gets -1.  One warp a token, the row in shared memory.
+// Order-preserving key of a logit; 0 stands for "not to be chosen" (minus infinity, NaN, taken).
+__device__ __forceinline__ uint32_t logit_key(float f) {
+    const uint32_t b = __float_as_uint(f + 0.0f);              // one zero
+    return f >= -FLT_MAX ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
+}
+__device__ __forceinline__ float key_logit(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+// Softmax over the experts and the k largest, ties to the lower index; the arithmetic of moe_route_kernel (moe.cu), so ids and
+// weights are those of dsl_moe_route.  One warp a token; `v`: room for a row of keys.  An entry without an expert gets -1.
 template <typename T>
-__device__ __forceinline__ void route_token(const Args& a, int t, float* v, const Plan& p, int lane) {
+__device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, const Plan& p, int lane) {
     const T* row = static_cast<const T*>(a.logits) + static_cast<size_t>(t) * a.experts;
-    float mx = -FLT_MAX;
-    for (int e = lane; e < a.experts; e += 32) {
-        const float f = static_cast<float>(row[e]);
-        v[e] = f;
-        mx = fmaxf(mx, f);
-    }
+    uint32_t keep[4];                                          // up to 128 experts stay in registers
+    const bool small = a.experts <= 128;
+    float mx, sum = 0.f;
+    if (small) {
+        float f[4];
+        uint32_t high = 0u;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-    float sum = 0.f;
-    for (int e = lane; e < a.experts; e += 32) sum += expf(v[e] - mx);
+        for (int i = 0; i < 4; ++i) {
+            f[i] = lane + 32 * i < a.experts ? static_cast<float>(row[lane + 32 * i]) : -FLT_MAX;
+            keep[i] = lane + 32 * i < a.experts ? logit_key(f[i]) : 0u;
+            high = max(high, keep[i]);
+        }
+        mx = key_logit(__reduce_max_sync(0xFFFFFFFFu, high));  // (nobody's to choose: no entry, whatever the sum)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < a.experts) sum += expf(f[i] - mx);
+    } else {
+        uint32_t high = 0u;
+        for (int e = lane; e < a.experts; e += 32) {
+            const float f = static_cast<float>(row[e]);
+            v[e] = __float_as_uint(f);
+            high = max(high, logit_key(f));
+        }
+        mx = key_logit(__reduce_max_sync(0xFFFFFFFFu, high));
+        for (int e = lane; e < a.experts; e += 32) {
+            const float f = __uint_as_float(v[e]);
+            sum += expf(f - mx);
+            v[e] = logit_key(f);
+        }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    __syncwarp();
-    float chosen_p = 0.f, psum = 0.f;
-    int chosen_e = -1;
+    uint32_t my_key = 0u;                                      // lane j keeps the j-th choice
+    int my_e = -1;
     for (int j = 0; j < a.k; ++j) {
-        // order-preserving keys: 0 stands for "not to be chosen"
         uint32_t best = 0u;
-        int bi = 0x7FFFFFFF;
-        for (int e = lane; e < a.experts; e += 32) {
-            const float f = v[e];
-            const uint32_t b = __float_as_uint(f + 0.0f);              // one zero
-            const uint32_t key = f >= -FLT_MAX ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
-            if (key > best) { best = key; bi = e; }
+        unsigned bi = 0x7FFFFFFFu;
+        if (small) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (keep[i] > best) { best = keep[i]; bi = lane + 32 * i; }
+        } else {
+            for (int e = lane; e < a.experts; e += 32) {
+                const uint32_t key = v[e];
+                if (key > best) { best = key; bi = e; }
+            }
         }
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-        if (top == 0u) break;                                          // uniform: nobody has one left
-        const int e = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, best == top ? static_cast<unsigned>(bi) : 0x7FFFFFFFu));
-        const float pr = __fdiv_rn(expf(v[e] - mx), sum);
-        psum += pr;
-        if (lane == j) { chosen_p = pr; chosen_e = e; }
-        __syncwarp();
-        if (lane == (e & 31)) v[e] = __uint_as_float(0xFF800000u);     // taken
-        __syncwarp();
+        if (top == 0u) break;                                  // uniform: nobody has one left
+        const int e = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, best == top ? bi : 0x7FFFFFFFu));
+        if (lane == j) { my_key = top; my_e = e; }
+        if (small) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e == lane + 32 * i) keep[i] = 0u;
+        } else if (lane == (e & 31)) {
+            v[e] = 0u;                                         // its own lane's alone to read
+        }
     }
+    const float pr = my_e >= 0 ? __fdiv_rn(expf(key_logit(my_key) - mx), sum) : 0.f;
+    float psum = 0.f;
+    for (int j = 0; j < a.k; ++j) psum += __shfl_sync(0xFFFFFFFFu, pr, j);
     if (lane < a.k) {
-        p.ids[t * a.k + lane] = chosen_e;
-        p.weights[t * a.k + lane] = a.renorm ? __fdiv_rn(chosen_p, psum) : chosen_p;
+        p.ids[t * a.k + lane] = my_e;
+        p.weights[t * a.k + lane] = a.renorm ? __fdiv_rn(pr, psum) : pr;
+        if (my_e >= 0) atomicOr(&p.tokens[my_e], 1u << t);
     }
 }
 
-// All threads.  `work`: WARPS * experts floats that nothing else uses yet.
-__device__ __forceinline__ void make_plan(const Args& a, Plan& p, float* work, int* s_segments) {
+// All threads.  `work`: WARPS * experts words that nothing else uses yet.
+__device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work, int* s_segments) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int e = threadIdx.x; e < a.experts; e += THREADS) p.count[e] = 0;
+    for (int e = threadIdx.x; e < a.experts; e += THREADS) p.tokens[e] = 0u;
+    __syncthreads();
     for (int t = warp; t < a.tokens; t += WARPS) {
         if (a.logits_dtype == DSL_F32) route_token<float>(a, t, work + warp * a.experts, p, lane);
         else route_token<__nv_bfloat16>(a, t, work + warp * a.experts, p, lane);
     }
     __syncthreads();
-    const int entries = a.tokens * a.k;
-    for (int i = threadIdx.x; i < entries; i += THREADS)
-        if (p.ids[i] >= 0) atomicAdd(&p.count[p.ids[i]], 1);           // counts: the order of the additions is nobody's business
-    __syncthreads();
     if (warp == 0) {
-        // experts 32 at a time: where an expert's rows begin, and its segments
+        // experts 32 at a time: their places and segments
         int rows = 0, segments = 0;
         for (int e0 = 0; e0 < a.experts; e0 += 32) {
             const int e = e0 + lane;
-            const int c = e < a.experts ? p.count[e] : 0;
+            const int c = e < a.experts ? __popc(p.tokens[e]) : 0;
             const int b = (c + a.block_rows - 1) / a.block_rows;
-            int rc = c, rb = b;
+            int run = c | (b << 16);                           // both sums at once: at most 1024 each
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int vc = __shfl_up_sync(0xFFFFFFFFu, rc, o), vb = __shfl_up_sync(0xFFFFFFFFu, rb, o);
-                if (lane >= o) { rc += vc; rb += vb; }
+                const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
+                if (lane >= o) run += v;
             }
-            if (e < a.experts) {
-                const int first = rows + rc - c;
-                p.count[e] = first;                                    // from here on: next free place of the expert
-                for (int i = 0; i < b; ++i) {
-                    const int s = segments + rb - b + i;
-                    p.seg_expert[s] = e;
-                    p.seg_first[s] = first + i * a.block_rows;
-                    p.seg_rows[s] = min(a.block_rows, c - i * a.block_rows);
-                }
+            const int first = rows + (run & 0xFFFF) - c, s0 = segments + (run >> 16) - b;
+            if (c > 0) p.base[e] = first;
+            for (int i = 0; i < b; ++i) {
+                p.seg_expert[s0 + i] = e;
+                p.seg_first[s0 + i] = first + i * a.block_rows;
+                p.seg_rows[s0 + i] = min(a.block_rows, c - i * a.block_rows);
             }
-            rows += __shfl_sync(0xFFFFFFFFu, rc, 31);
-            segments += __shfl_sync(0xFFFFFFFFu, rb, 31);
-        }
-        __syncwarp();
-        for (int i0 = 0; i0 < entries; i0 += 32) {                     // stable: every CTA makes the same list
-            const int i = i0 + lane;
-            const int e = i < entries ? p.ids[i] : -1;
-            const unsigned peers = __match_any_sync(0xFFFFFFFFu, e);
-            const int leader = __ffs(peers) - 1;
-            int base = 0;
-            if (e >= 0 && lane == leader) {
-                base = p.count[e];
-                p.count[e] = base + __popc(peers);
-            }
-            base = __shfl_sync(0xFFFFFFFFu, base, leader);
-            if (e >= 0) p.order[base + __popc(peers & ((1u << lane) - 1u))] = i;
-            __syncwarp();
+            run = __shfl_sync(0xFFFFFFFFu, run, 31);
+            rows += run & 0xFFFF;
+            segments += run >> 16;
         }
         if (lane == 0) *s_segments = segments;
+    }
+    __syncthreads();
+    for (int t = warp; t < a.tokens; t += WARPS) {
+        const int e = lane < a.k ? p.ids[t * a.k + lane] : -1;
+        if (e >= 0) p.order[p.base[e] + __popc(p.tokens[e] & ((1u << t) - 1u))] = t * a.k + lane;
     }
     __syncthreads();
     p.segments = *s_segments;
@@ -236,136 +275,166 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
     return r;
 }
 
-// What a lane holds of one step: rows g and g + 8, four chunks, with the scales of its pieces.
+__device__ __forceinline__ uint4 load_table(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : (j == 1 ? v.y : (j == 2 ? v.z : v.w)); }
+
+// What a lane holds of one step: 16 bytes of each of its four rows (g + 32 j of the tile), with the scales.
 template <int FMT>
 struct Piece {
-    uint4 w[2][4];
-    uint32_t s[FMT == NV || FMT == MX ? 2 : 1][FMT == F8G ? 2 : 4];      // NV: two UE4M3 bytes; MX: one E8M0 byte; F8G: fp32 of a 128-group
+    static constexpr bool TABLE = FMT == NV || FMT == MX;
+    uint4 w[4];
+    uint4 s;                             // NV, MX: word j = the scale bytes of row j's atom
+    float group;                         // F8G: scale of the step's 128-element group
 
-    __device__ __forceinline__ void load(const Args& a, const uint8_t* row0, const uint8_t* row1, const uint8_t* sc0, const uint8_t* sc1,
-                                         int step, int t) {
+    // `row`: row j = 0 of this lane, `pitch`: 32 rows on; `rows`: bit j = row j exists and is this CTA's
+    __device__ __forceinline__ void load(const Args& a, const uint8_t* row, int pitch, unsigned rows, const uint8_t* scale, int step, int t) {
+        const int at = step * STEP + t * 16;
+        const bool in = at < a.row_bytes;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int at = step * STEP + c * 64 + t * 16;
-            const bool in = at < a.row_bytes;
-            w[0][c] = in ? load_stream(row0 + at) : make_uint4(0u, 0u, 0u, 0u);
-            w[1][c] = in ? load_stream(row1 + at) : make_uint4(0u, 0u, 0u, 0u);
-            if (FMT == NV) {             // blocks 2 * (16-byte piece), + 1: atom piece / 2, bytes (piece % 2) * 2
-                const int piece = at >> 4;
-                const size_t o = static_cast<size_t>(piece >> 1) * 512 + (piece & 1) * 2;
-                s[0][c] = in ? __ldg(reinterpret_cast<const unsigned short*>(sc0 + o)) : 0u;
-                s[1][c] = in ? __ldg(reinterpret_cast<const unsigned short*>(sc1 + o)) : 0u;
-            }
-            if (FMT == MX) {             // block = 16-byte piece
-                const int piece = at >> 4;
-                const size_t o = static_cast<size_t>(piece >> 2) * 512 + (piece & 3);
-                s[0][c] = in ? __ldg(sc0 + o) : 0u;
-                s[1][c] = in ? __ldg(sc1 + o) : 0u;
-            }
-            if (FMT == F8G && c % 2 == 0)      // sc0: this tile's row of block scales
-                s[0][c / 2] = in ? __float_as_uint(__ldg(reinterpret_cast<const float*>(sc0) + (step * STEP + c * 64) / 128)) : 0u;
+        for (int j = 0; j < 4; ++j) {
+            w[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (in && (rows >> j & 1u)) w[j] = load_stream(row + static_cast<size_t>(static_cast<unsigned>(j * pitch)) + at);
         }
+        // NV: two blocks a piece, so atom piece / 2; MX: one, atom piece / 4, which all lanes of a quad need for its maximum
+        if (FMT == NV) s = in ? load_table(scale + static_cast<size_t>(at >> 5) * 512) : make_uint4(0u, 0u, 0u, 0u);
+        if (FMT == MX) s = step * STEP < a.row_bytes ? load_table(scale + static_cast<size_t>(step) * 512) : make_uint4(0u, 0u, 0u, 0u);
+        if (FMT == F8G) group = step * STEP < a.row_bytes ? __ldg(reinterpret_cast<const float*>(scale) + (step >> 1)) : 0.f;
     }
 };
 
-// Sums of one step: acc[nt] += weights (16 rows) x the rows in shared memory (columns nt * 8 ...).  `b`: this lane's place in them.
-template <int FMT, int NT>
-__device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t* const (&b)[NT], int step, int nt_used, int parts, int part_bytes,
-                                              float (&acc)[NT][4]) {
+// A fragment of two k16 steps from vector v of a lane's pieces of two rows (16 consecutive values of eight lanes' rows ...): the
+// widened weights as they are, without FP4 scales.
+template <int FMT>
+__device__ __forceinline__ void widen_rows(const uint4& q0, const uint4& q1, int v, uint32_t (&a0)[4], uint32_t (&a1)[4]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const uint4& q = r == 0 ? q0 : q1;
+        if (FMT == BF) {
+            a0[r] = q.x; a0[r + 2] = q.y; a1[r] = q.z; a1[r + 2] = q.w;
+        } else if (FMT == F8 || FMT == F8G) {
+            const uint32_t w0 = word(q, 2 * v), w1 = word(q, 2 * v + 1);
+            a0[r] = widen_e4m3(w0);
+            a0[r + 2] = widen_e4m3(w0 >> 16);
+            a1[r] = widen_e4m3(w1);
+            a1[r + 2] = widen_e4m3(w1 >> 16);
+        } else if (FMT == I8) {
+            const uint32_t w0 = word(q, 2 * v) ^ 0x80808080u, w1 = word(q, 2 * v + 1) ^ 0x80808080u;
+            a0[r] = widen_int8(w0, 0x4140);
+            a0[r + 2] = widen_int8(w0, 0x4342);
+            a1[r] = widen_int8(w1, 0x4140);
+            a1[r + 2] = widen_int8(w1, 0x4342);
+        } else {
+            const uint32_t w = word(q, v);
+            a0[r] = widen_e2m1<0>(w);
+            a0[r + 2] = widen_e2m1<1>(w);
+            a1[r] = widen_e2m1<2>(w);
+            a1[r + 2] = widen_e2m1<3>(w);
+        }
+    }
+}
+
+// Sums of one step, columns = rows of the activations: acc[m * 4 ..] += weights (rows g + 64 m and g + 64 m + 32) x the rows in
+// shared memory (eight columns).  `b`: this lane's place in them.  NVFP4's scales are multiplied into the weights (exactly).
+template <int FMT>
+__device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t* b, int step, int t, int parts, int part_bytes, float (&acc)[8]) {
     using F = Fmt<FMT>;
     constexpr int VECS = F::ELEMS / 8;                  // 16-byte vectors of activations against one 16-byte piece of weights
-    constexpr bool APART = FMT == F8G || FMT == MX;     // chunk sums are scaled before they are added
-    float sum[NT][4];
+    float sum[2][4];                                    // F8G: scaled before they are added
+    uint32_t hs[4][2];                                  // NV: f16 scales of this lane's two blocks, by row
+    if (FMT == NV) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if (APART && (FMT == MX || c % 2 == 0)) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t two = widen_e4m3(word(p.s, j) >> ((t & 1) * 16));
+            hs[j][0] = __byte_perm(two, two, 0x1010);
+            hs[j][1] = __byte_perm(two, two, 0x3232);
         }
-        uint32_t hs[2][2];           // f16 scales of this lane's blocks (NV: two a piece, MX: one)
-        float top[2];                // MX: the chunk's largest scale of either row
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[m][j] = FMT == F8G ? 0.f : acc[m * 4 + j];
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        const uint8_t* at = b + (step * VECS + v) * 64;
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        uint4 lo;
+        if (F::PARTS == 2 && parts == 2) lo = *reinterpret_cast<const uint4*>(at + part_bytes);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t a0[4], a1[4];
+            widen_rows<FMT>(p.w[2 * m], p.w[2 * m + 1], v, a0, a1);
+            if (FMT == NV) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a0[i] = hmul2(a0[i], hs[2 * m + (i & 1)][v / 2]);
+                    a1[i] = hmul2(a1[i], hs[2 * m + (i & 1)][v / 2]);
+                }
+            }
+            mma16<F::BF16>(sum[m], a0, x.x, x.y);
+            mma16<F::BF16>(sum[m], a1, x.z, x.w);
+            if (F::PARTS == 2 && parts == 2) {
+                mma16<F::BF16>(sum[m], a0, lo.x, lo.y);
+                mma16<F::BF16>(sum[m], a1, lo.z, lo.w);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[m * 4 + j] = FMT == F8G ? fmaf(sum[m][j], p.group, acc[m * 4 + j]) : sum[m][j];
+}
+
+// Sums of one step, columns = scale blocks, for FP4 weights against few rows: a step has eight (NVFP4) or four (MXFP4) blocks along
+// K, and B holds a row's values in the column of their block alone (zeros elsewhere), so that column n of the product is block n's
+// sum and its scale meets one fp32 number instead of sixteen weights - half of the instructions that the widening above takes.
+// Lane t holds blocks 2 t and 2 t + 1, as values and as columns (NVFP4), or block t, and columns t % 2 * 2 and + 1 (MXFP4).
+// acc[set * 4 + j]: row j of the weights, of the lane's columns; a set is a row (NVFP4) or two rows (MXFP4) of the activations.
+// `b`: per set and half of a piece, this lane's place in its row or in the row of zeros.
+template <int FMT, int SETS>
+__device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* const (&b)[SETS][2], int step, int t, float (&acc)[8]) {
+    float sum[SETS][2][4];
+#pragma unroll
+    for (int k = 0; k < SETS; ++k)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[k][m][j] = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint4 x[SETS];
+#pragma unroll
+        for (int k = 0; k < SETS; ++k) x[k] = *reinterpret_cast<const uint4*>(b[k][FMT == NV ? v / 2 : 0] + (step * 4 + v) * 64);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t a0[4], a1[4];
+            widen_rows<FMT>(p.w[2 * m], p.w[2 * m + 1], v, a0, a1);
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                mma16<false>(sum[k][m], a0, x[k].x, x[k].y);
+                mma16<false>(sum[k][m], a1, x[k].z, x[k].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t two = word(p.s, j) >> ((t & 1) * 16);
+        float s0, s1;
         if (FMT == NV) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t two = widen_e4m3(p.s[r][c]);
-                hs[r][0] = __byte_perm(two, two, 0x1010);
-                hs[r][1] = __byte_perm(two, two, 0x3232);
-            }
-        }
-        if (FMT == MX) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t e = p.s[r][c];
-                uint32_t m = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, 1));
-                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-                // 2^(e - m) in f16: normal down to 2^-14, then 2^-24 at the least, 0 below (under a 2^-24th of the chunk's largest)
-                const int d = static_cast<int>(m - e);
-                const uint32_t one = d < 15 ? static_cast<uint32_t>(15 - d) << 10 : (d < 25 ? 1u << (24 - d) : 0u);
-                hs[r][0] = one | (one << 16);
-                // byte 255 is NaN; 2^(m - 127) for m = 0 is subnormal
-                top[r] = m == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(m == 0u ? 0x00400000u : m << 23);
-            }
+            const uint32_t h = widen_e4m3(two);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            s0 = f.x;
+            s1 = f.y;
+        } else {
+            // 2^(byte - 127): the byte as an exponent, subnormal for 0, and 255 (infinity so far) is NaN
+            s0 = __uint_as_float(max((two & 255u) << 23, 0x00400000u));
+            s1 = __uint_as_float(max((two >> 8 & 255u) << 23, 0x00400000u));
+            s0 = fmaf(0.0f, s0, s0);
+            s1 = fmaf(0.0f, s1, s1);
         }
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-            uint4 x[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-                if (i < nt_used) x[i] = *reinterpret_cast<const uint4*>(b[i] + ((step * 4 + c) * VECS + v) * 64);
-            uint32_t a[2][2][2];     // [k16 step][row half][k half]
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint4 q = p.w[r][c];
-                if (FMT == BF) {
-                    a[0][r][0] = q.x; a[0][r][1] = q.y; a[1][r][0] = q.z; a[1][r][1] = q.w;
-                } else if (FMT == F8 || FMT == F8G) {
-                    const uint32_t w0 = v == 0 ? q.x : q.z, w1 = v == 0 ? q.y : q.w;
-                    a[0][r][0] = widen_e4m3(w0);
-                    a[0][r][1] = widen_e4m3(w0 >> 16);
-                    a[1][r][0] = widen_e4m3(w1);
-                    a[1][r][1] = widen_e4m3(w1 >> 16);
-                } else if (FMT == I8) {
-                    const uint32_t w0 = (v == 0 ? q.x : q.z) ^ 0x80808080u, w1 = (v == 0 ? q.y : q.w) ^ 0x80808080u;
-                    a[0][r][0] = widen_int8(w0, 0x4140);
-                    a[0][r][1] = widen_int8(w0, 0x4342);
-                    a[1][r][0] = widen_int8(w1, 0x4140);
-                    a[1][r][1] = widen_int8(w1, 0x4342);
-                } else {
-                    const uint32_t w0 = v == 0 ? q.x : (v == 1 ? q.y : (v == 2 ? q.z : q.w));
-                    const uint32_t f = FMT == NV ? hs[r][v / 2] : hs[r][0];
-                    a[0][r][0] = hmul2(widen_e2m1<0>(w0), f);
-                    a[0][r][1] = hmul2(widen_e2m1<1>(w0), f);
-                    a[1][r][0] = hmul2(widen_e2m1<2>(w0), f);
-                    a[1][r][1] = hmul2(widen_e2m1<3>(w0), f);
-                }
-            }
-            const uint32_t a0[4] = {a[0][0][0], a[0][1][0], a[0][0][1], a[0][1][1]};
-            const uint32_t a1[4] = {a[1][0][0], a[1][1][0], a[1][0][1], a[1][1][1]};
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                if (i < nt_used) {
-                    float(&d)[4] = APART ? sum[i] : acc[i];
-                    mma16<F::BF16>(d, a0, x[i].x, x[i].y);
-                    mma16<F::BF16>(d, a1, x[i].z, x[i].w);
-                    if (F::PARTS == 2 && parts == 2) {
-                        const uint4 lo = *reinterpret_cast<const uint4*>(b[i] + part_bytes + ((step * 4 + c) * VECS + v) * 64);
-                        mma16<F::BF16>(d, a0, lo.x, lo.y);
-                        mma16<F::BF16>(d, a1, lo.z, lo.w);
-                    }
-                }
-            }
-        }
-        if (APART && (FMT == MX || c % 2 == 1)) {
-            const float t0 = FMT == MX ? top[0] : __uint_as_float(p.s[0][c / 2]), t1 = FMT == MX ? top[1] : t0;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                acc[i][0] = fmaf(sum[i][0], t0, acc[i][0]);
-                acc[i][1] = fmaf(sum[i][1], t0, acc[i][1]);
-                acc[i][2] = fmaf(sum[i][2], t1, acc[i][2]);
-                acc[i][3] = fmaf(sum[i][3], t1, acc[i][3]);
-            }
+        for (int k = 0; k < SETS; ++k) {
+            acc[k * 4 + j] = fmaf(sum[k][j >> 1][(j & 1) * 2], s0, acc[k * 4 + j]);
+            acc[k * 4 + j] = fmaf(sum[k][j >> 1][(j & 1) * 2 + 1], s1, acc[k * 4 + j]);
         }
     }
 }
@@ -401,86 +470,86 @@ __device__ __forceinline__ float row_factor(uint32_t amax, float* inverse) {
     *inverse = __uint_as_float(static_cast<uint32_t>(127 - s) << 23);
     return __uint_as_float(static_cast<uint32_t>(127 + s) << 23);
 }
+// Rows whose largest magnitude lies here are taken as they are: f16 holds 16-bit values down to 2^-17 exactly and is off by
+// 2^-25 at most below, 2^-25 of the largest.  Normed activations do.
+__device__ __forceinline__ bool fits_f16(uint32_t amax) { return amax >= __float_as_uint(1.0f) && amax < __float_as_uint(32768.0f); }
 
-// Rows seg_first .. + rows of the list; element j of a row lies in chunk j / (4 E), lane t = j / E % 4, vector j % E / 8, i.e. at
-// ((chunk * E / 8 + vector) * 4 + t) * 16 bytes.  Elements past the row's end up to whole steps are zeros.
+// Rows first .. first + rows of the list; element j of a row lies in step j / (4 E), lane t = j / E % 4, vector j % E / 8, i.e. at
+// ((step * E / 8 + vector) * 4 + t) * 16 bytes.  Elements past the row's end up to whole steps are zeros; with FP4 weights a row of
+// zeros follows the last one.  One look at the rows, a second one where some have to be scaled (`scaled`: they may have to be).
 template <int FMT, bool DOWN>
 __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int first, int rows, uint8_t* dst, int pitch, int part_bytes,
-                                           uint32_t* s_amax, float* s_inverse) {
+                                           bool scaled, uint32_t* s_amax, float* s_inverse) {
     using F = Fmt<FMT>;
     constexpr int VECS = F::ELEMS / 8;
     const int vectors = a.steps * (STEP / 16) * VECS;                 // 8-element vectors of a padded row
     const int dtype = DOWN ? DSL_F32 : a.x_dtype;
-    auto source = [&](int r) {
-        const int entry = p.order[first + r];
-        return static_cast<size_t>(DOWN ? entry : entry / a.k) * a.kdim;
-    };
-    // f16 rows are what they are, bf16 ones as bf16 too; the second bf16 term of an fp32 value wants room below the first
-    const bool scaled = dtype == DSL_F32 || (dtype == DSL_BF16 && !F::BF16);
-    if (threadIdx.x < rows) {
-        s_amax[threadIdx.x] = 0u;
-        s_inverse[threadIdx.x] = 1.0f;
-    }
+    if (threadIdx.x < rows) s_amax[threadIdx.x] = 0u;
     __syncthreads();
-    if (scaled) {
+    for (bool again = false;; again = true) {
+        bool more = false;
         for (int r = 0; r < rows; ++r) {
-            const size_t src = source(r);
+            const int entry = p.order[first + r];
+            const size_t src = static_cast<size_t>(DOWN ? entry : quotient(entry, a.k, a.div_k)) * a.kdim;
+            float factor = 1.0f, inverse = 1.0f;
+            if (again) {
+                if (fits_f16(s_amax[r])) continue;
+                factor = row_factor(s_amax[r], &inverse);
+            }
+            if (threadIdx.x == 0) s_inverse[r] = inverse;
             uint32_t m = 0u;
-            for (int v = threadIdx.x; v * 8 < a.kdim; v += THREADS) {
+#pragma unroll 4
+            for (int v = threadIdx.x; v < vectors; v += THREADS) {
                 float f[8];
-                load8(a.x, dtype, src + v * 8, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-            }
-            m = __reduce_max_sync(0xFFFFFFFFu, m);
-            if ((threadIdx.x & 31) == 0 && m != 0u) atomicMax(&s_amax[r], m);
-        }
-        __syncthreads();
-    }
-    for (int r = 0; r < rows; ++r) {
-        const size_t src = source(r);
-        float inverse = 1.0f;
-        const float factor = scaled ? row_factor(s_amax[r], &inverse) : 1.0f;
-        if (scaled && threadIdx.x == 0) s_inverse[r] = inverse;
-        for (int v = threadIdx.x; v < vectors; v += THREADS) {
-            float f[8];
-            if (v * 8 < a.kdim) {
-                load8(a.x, dtype, src + v * 8, f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = 0.f;
-            }
-            const int piece = v / VECS;
-            uint8_t* d = dst + static_cast<size_t>(r) * pitch + (((piece >> 2) * VECS + v % VECS) * 4 + (piece & 3)) * 16;
-            uint32_t w[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (F::BF16) {
-                    const float f0 = f[2 * i] * factor, f1 = f[2 * i + 1] * factor;
-                    const __nv_bfloat162 hi = __floats2bfloat162_rn(f0, f1);
-                    const float h0 = __low2float(hi), h1 = __high2float(hi);       // an infinity leaves no rest
-                    const __nv_bfloat162 rest = __floats2bfloat162_rn(isinf(h0) ? 0.f : f0 - h0, isinf(h1) ? 0.f : f1 - h1);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&hi);
-                    lo[i] = *reinterpret_cast<const uint32_t*>(&rest);
+                if (v * 8 < a.kdim) {
+                    load8(a.x, dtype, src + v * 8, f);
                 } else {
-                    const __half2 h = __floats2half2_rn(f[2 * i] * factor, f[2 * i + 1] * factor);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = 0.f;
                 }
+                const int piece = v / VECS;
+                uint8_t* d = dst + static_cast<size_t>(r) * pitch + (((piece >> 2) * VECS + v % VECS) * 4 + (piece & 3)) * 16;
+                uint32_t w[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f0 = f[2 * i] * factor, f1 = f[2 * i + 1] * factor;
+                    m = max(m, max(__float_as_uint(f[2 * i]) & 0x7FFFFFFFu, __float_as_uint(f[2 * i + 1]) & 0x7FFFFFFFu));
+                    if (F::BF16) {
+                        const __nv_bfloat162 hi = __floats2bfloat162_rn(f0, f1);
+                        const float h0 = __low2float(hi), h1 = __high2float(hi);       // an infinity leaves no rest
+                        const __nv_bfloat162 rest = __floats2bfloat162_rn(isinf(h0) ? 0.f : f0 - h0, isinf(h1) ? 0.f : f1 - h1);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&hi);
+                        lo[i] = *reinterpret_cast<const uint32_t*>(&rest);
+                    } else {
+                        const __half2 h = __floats2half2_rn(f0, f1);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+                *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (F::PARTS == 2 && a.parts == 2) *reinterpret_cast<uint4*>(d + part_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
-            *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (F::PARTS == 2 && a.parts == 2) *reinterpret_cast<uint4*>(d + part_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (scaled && !again) {
+                m = __reduce_max_sync(0xFFFFFFFFu, m);
+                if ((threadIdx.x & 31) == 0 && m != 0u) atomicMax(&s_amax[r], m);
+            }
         }
+        if (F::FP4 && !again)
+            for (int v = threadIdx.x; v < part_bytes / 16; v += THREADS)
+                *reinterpret_cast<uint4*>(dst + static_cast<size_t>(rows) * pitch + v * 16) = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+        if (!scaled || again) return;
+        for (int r = 0; r < rows; ++r) more |= !fits_f16(s_amax[r]);
+        if (!more) return;
     }
-    __syncthreads();
 }
 
 // ---- shared memory ----------------------------------------------------------------------------------------------------------------
 struct Layout {
-    int ids, weights, order, seg_expert, seg_first, seg_rows, count, misc, red, rows, total;
+    int ids, weights, order, seg_expert, seg_first, seg_rows, chosen, base, misc, sums, rows, total;
     int pitch, part_bytes;
 };
-// `elems`: elements of a weight in 16 bytes; the rows' region doubles as the router's room.
-__host__ __device__ inline Layout layout_of(const Args& a, int elems, int nt) {
+// `elems`: elements of a weight in 16 bytes; the rows' region doubles as the router's room and the list of finished units.
+__host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) {
     Layout l;
     const int entries = a.tokens * a.k;
     int at = 0;
@@ -491,31 +560,34 @@ __host__ __device__ inline Layout layout_of(const Args& a, int elems, int nt) {
     l.seg_expert = take(entries * 4);
     l.seg_first = take(entries * 4);
     l.seg_rows = take(entries * 4);
-    l.count = take(a.experts * 4);
-    l.misc = take(32 + 32 * 8);                                        // segments, flags; amax and inverse factor of 16 rows
-    l.red = take(2 * WARPS * nt * 8 * RED_PITCH * 4);
-    l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 256
+    l.chosen = take(a.experts * 4);
+    l.base = take(a.experts * 4);
+    l.misc = take(16 + 2 * 8 * 4);                                     // two counters; amax of the rows, their inverse factors
+    l.sums = take(3 * WARPS * SUM_FLOATS * 4);                         // a run's first piece of a tile, its last one, a whole one
+    l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 128
     l.pitch = l.part_bytes * a.parts + 64;                             // two rows start half a bank round apart
     l.rows = take(0);
-    const int rows = a.block_rows * l.pitch, room = WARPS * a.experts * 4;
-    l.total = l.rows + (rows > room ? rows : room);
+    int room = (a.block_rows + (fp4 ? 1 : 0)) * l.pitch;
+    if (room < WARPS * a.experts * 4) room = WARPS * a.experts * 4;
+    if (room < a.units * 4) room = a.units * 4;
+    l.total = l.rows + room;
     return l;
 }
 
-__device__ __forceinline__ void group_sync(int group, int split) {
-    if (split == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(split * 32) : "memory");
-}
+template <int N> struct Way { static constexpr int value = N; };
+
+// Row j (of four) of unit pair `tile` that belongs to lane group g.
+__device__ __forceinline__ int row_of(int tile, int g, int j) { return (tile >> 2) * 128 + (tile & 3) * 8 + g + 32 * j; }
 
 }  // namespace md
 
-template <int FMT, int NT, bool DOWN>
+template <int FMT, bool DOWN>
 __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Args a) {
     using F = md::Fmt<FMT>;
     using md::THREADS;
     using md::WARPS;
     extern __shared__ __align__(16) uint8_t smem[];
-    const md::Layout l = md::layout_of(a, F::ELEMS, NT);
+    const md::Layout l = md::layout_of(a, F::ELEMS, F::FP4);
     md::Plan plan;
     plan.ids = reinterpret_cast<int*>(smem + l.ids);
     plan.weights = reinterpret_cast<float*>(smem + l.weights);
@@ -523,11 +595,12 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     plan.seg_expert = reinterpret_cast<int*>(smem + l.seg_expert);
     plan.seg_first = reinterpret_cast<int*>(smem + l.seg_first);
     plan.seg_rows = reinterpret_cast<int*>(smem + l.seg_rows);
-    plan.count = reinterpret_cast<int*>(smem + l.count);
-    int* s_misc = reinterpret_cast<int*>(smem + l.misc);
-    uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + l.misc + 32);
-    float* s_inverse = reinterpret_cast<float*>(smem + l.misc + 32 + 64);
-    float* s_red = reinterpret_cast<float*>(smem + l.red);
+    plan.tokens = reinterpret_cast<uint32_t*>(smem + l.chosen);
+    plan.base = reinterpret_cast<int*>(smem + l.base);
+    int* s_misc = reinterpret_cast<int*>(smem + l.misc);               // [0] segments, [1] units that this CTA completes
+    uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + l.misc + 16);
+    float* s_inverse = reinterpret_cast<float*>(smem + l.misc + 16 + 32);
+    float* s_sums = reinterpret_cast<float*>(smem + l.sums);
     uint8_t* s_rows = smem + l.rows;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -539,142 +612,200 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         if (blockIdx.x == 0)
             for (int i = threadIdx.x; i < a.arrived_count; i += THREADS) a.arrived[i] = 0;
     }
+    // f16 rows are what they are, bf16 ones as bf16 too; the second bf16 term of an fp32 value wants room below the first
+    const bool scaled = DOWN || a.x_dtype == DSL_F32 || (a.x_dtype == DSL_BF16 && !F::BF16);
     // Down may get this far while up still runs: logits and weights were complete before up started.
-    md::make_plan(a, plan, reinterpret_cast<float*>(s_rows), s_misc);
-    const long long items = static_cast<long long>(plan.segments) * a.tiles;
-    const long long begin = items * blockIdx.x / gridDim.x, end = items * (blockIdx.x + 1) / gridDim.x;
-
-    const int groups = WARPS / a.split, group = warp / a.split, slice = warp - group * a.split;
-    const int my_steps = (a.steps - slice + a.split - 1) / a.split;
-    float* red = s_red + warp * (NT * 8 * md::RED_PITCH);
-    const float* red_group = s_red + group * a.split * (NT * 8 * md::RED_PITCH);
-    constexpr int RED_ALL = WARPS * NT * 8 * md::RED_PITCH;
-    int parity = 0;
+    md::make_plan(a, plan, reinterpret_cast<uint32_t*>(s_rows), s_misc);
+    // The list of work: every expert's units behind entry_cost places without work, so that a CTA which passes from one expert to
+    // the next, and has to fetch that one's rows, is dealt less.
+    const int span = a.units + a.entry_cost, items = plan.segments * span;
+    const int ctas = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
+    const int share = md::quotient(items, ctas, a.div_grid), more_than = items - share * ctas;
+    const int begin = bid * share + min(bid, more_than), end = begin + share + (bid < more_than ? 1 : 0);
     bool waited = !DOWN;
 
-    for (long long item = begin; item < end;) {
-        const int seg = static_cast<int>(item / a.tiles);
-        const int tile0 = static_cast<int>(item - static_cast<long long>(seg) * a.tiles);
-        const int tile1 = static_cast<int>(min(static_cast<long long>(a.tiles), tile0 + (end - item)));
+    for (int item = begin; item < end;) {
+        const int seg = md::quotient(item, span, a.div_span);
+        const int off0 = item - seg * span, off1 = min(span, off0 + (end - item));
+        item += off1 - off0;
+        const int unit0 = max(0, off0 - a.entry_cost), unit1 = max(0, off1 - a.entry_cost);
+        if (unit0 == unit1) continue;
         const int expert = plan.seg_expert[seg], first = plan.seg_first[seg], rows = plan.seg_rows[seg];
-        item += tile1 - tile0;
+        // this CTA's tiles of the expert, and this warp's run of their steps
+        const int tile0 = unit0 >> 1, tiles = ((unit1 + 1) >> 1) - tile0;
+        const int all = tiles * a.steps;
+        const int run0 = all * warp / WARPS, run1 = all * (warp + 1) / WARPS;
+        int at = run0, tile = md::quotient(run0, a.steps, a.div_steps), step = run0 - tile * a.steps;      // tile counts from tile0
 
-        // this warp's tiles: tile0 + group, + groups, ...; a tile's steps: slice, + split, ...
-        int tile = tile0 + group, step = slice;
-        const uint8_t *row0, *row1, *sc0 = nullptr, *sc1 = nullptr;
+        // Where the loads are: up to AHEAD - 1 steps before the products.
+        static_assert(F::AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
+        const int pitch = 32 * a.row_bytes;
+        int l_at = run0, l_step = step, l_tile = tile0 + tile;
+        const uint8_t *l_row = nullptr, *l_scale = nullptr;
+        unsigned l_rows = 0;
         auto locate = [&]() {
-            const int r0 = min(tile * 16 + g, a.n - 1), r1 = min(tile * 16 + g + 8, a.n - 1);       // rows past the end: any that exist
-            row0 = a.w + (static_cast<size_t>(expert) * a.n + r0) * a.row_bytes;
-            row1 = a.w + (static_cast<size_t>(expert) * a.n + r1) * a.row_bytes;
-            if (FMT == md::NV || FMT == md::MX) {
-                const size_t t128 = static_cast<size_t>(expert) * ((a.n + 127) / 128);
-                sc0 = a.scale + (t128 + r0 / 128) * a.katoms * 512 + (r0 % 32) * 16 + (r0 % 128) / 32 * 4;
-                sc1 = a.scale + (t128 + r1 / 128) * a.katoms * 512 + (r1 % 32) * 16 + (r1 % 128) / 32 * 4;
+            const int r0 = md::row_of(l_tile, g, 0);
+            l_row = a.w + (static_cast<size_t>(expert) * a.n + r0) * a.row_bytes;
+            const unsigned in = r0 >= a.n ? 0u : min(4u, static_cast<unsigned>(a.n - r0 + 31) / 32u);      // rows that the weight has
+            l_rows = ((1u << in) - 1u) & (2 * l_tile < unit0 ? 0xCu : 0xFu) & (2 * l_tile + 1 >= unit1 ? 0x3u : 0xFu);
+            const size_t block = static_cast<size_t>(expert) * ((a.n + 127) / 128) + (l_tile >> 2);
+            if (FMT == md::NV || FMT == md::MX) l_scale = a.scale + block * a.katoms * 512 + ((l_tile & 3) * 8 + g) * 16;
+            if (FMT == md::F8G) l_scale = a.scale + block * (a.kdim / 128) * 4;
+        };
+        md::Piece<FMT> buf[F::AHEAD];
+        auto fetch = [&](md::Piece<FMT>& p) {
+            if (l_at < run1) {
+                p.load(a, l_row, pitch, l_rows, l_scale, l_step, t4);
+                ++l_at;
+                if (++l_step == a.steps) {
+                    l_step = 0;
+                    ++l_tile;
+                    locate();
+                }
             }
-            if (FMT == md::F8G)
-                sc0 = a.scale + (static_cast<size_t>(expert) * ((a.n + 127) / 128) + tile / 8) * (a.kdim / 128) * 4;
         };
-        // moves on to this warp's next step; false past the last one
-        auto advance = [&](int& tl, int& st) {
-            st += a.split;
-            if (st >= a.steps) { st = slice; tl += groups; }
-            return tl < tile1;
-        };
-        md::Piece<FMT> even, odd;
-        bool more = tile < tile1 && my_steps > 0;
-        if (more) {
-            locate();
-            even.load(a, row0, row1, sc0, sc1, step, t4);
-        }
+        if (run0 < run1) locate();
+#pragma unroll
+        for (int i = 0; i + 1 < F::AHEAD; ++i) fetch(buf[i]);
         if (!waited) {           // the hidden activation is up's
             griddep_wait();
             griddep_launch_dependents();
             waited = true;
         }
-        __syncthreads();         // the rows of the segment before are read, the router's room is free
-        md::stage_rows<FMT, DOWN>(a, plan, first, rows, s_rows, l.pitch, l.part_bytes, s_amax, s_inverse);
-        const int nt_used = NT == 1 ? 1 : (rows + 7) / 8;
-        const uint8_t* b[NT];
+        __syncthreads();         // the segment before is finished, the router's room is free
+        md::stage_rows<FMT, DOWN>(a, plan, first, rows, s_rows, l.pitch, l.part_bytes, scaled, s_amax, s_inverse);
+        float acc[8];
+        auto clear = [&]() {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) b[i] = s_rows + static_cast<size_t>(min(i * 8 + g, rows - 1)) * l.pitch + t4 * 16;
-        float acc[NT][4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-
-        // the sums of a finished tile: over the group's warps, in order, then scales and the activation
-        auto finish = [&](int done) {
-            float* mine = red + parity * RED_ALL;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                if (i < nt_used) {
-                    float* c = mine + (i * 8 + 2 * t4) * md::RED_PITCH + g;
-                    c[0] = acc[i][0];
-                    c[md::RED_PITCH] = acc[i][1];
-                    c[8] = acc[i][2];
-                    c[md::RED_PITCH + 8] = acc[i][3];
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-            }
-            md::group_sync(group, a.split);
-            const float* theirs = red_group + parity * RED_ALL;
-            parity ^= 1;
-            auto total = [&](int col, int row) {
-                float s = 0.f;
-                for (int w = 0; w < a.split; ++w) s += theirs[w * (NT * 8 * md::RED_PITCH) + col * md::RED_PITCH + row];
-                s *= s_inverse[col];
-                if (FMT == md::F8) s *= *reinterpret_cast<const float*>(a.scale);
-                if (FMT == md::NV) s *= *a.global_scale;
-                if (FMT == md::I8) s *= reinterpret_cast<const float*>(a.scale)[static_cast<size_t>(expert) * a.n + min(done * 16 + row, a.n - 1)];
-                return s;
-            };
-            const int me = slice * 32 + lane, all = a.split * 32;
-            if (DOWN) {
-                for (int i = me; i < rows * 16; i += all) {
-                    const int col = i >> 4, row = i & 15;
-                    if (done * 16 + row < a.n) a.y[static_cast<size_t>(plan.order[first + col]) * a.n + done * 16 + row] = total(col, row);
-                }
+            for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+        };
+        clear();
+        // The sums of a tile that ends, or of the piece of it that the run has, go to one of the warp's three places in shared
+        // memory: 0 a tile that begins before the run, 1 one that ends behind it, 2 a whole one, which is finished at once.
+        float* mine = s_sums + warp * (3 * md::SUM_FLOATS);
+        // Everything from here to the segment's end, for one way of forming the products (sets: 0 rows as columns, else blocks).
+        auto stream = [&](auto way) {
+            constexpr int SETS = decltype(way)::value;
+            constexpr int HELD = SETS > 0 ? SETS : 1;
+            const uint8_t* b[HELD][2];
+            if (SETS == 0) {
+                b[0][0] = b[0][1] = s_rows + static_cast<size_t>(min(g, rows - 1)) * l.pitch + t4 * 16;      // columns past the rows: any
             } else {
-                for (int i = me; i < rows * 8; i += all) {
-                    const int col = i >> 3, j = i & 7;
-                    if (done * 16 + 2 * j + 1 < a.n) {
-                        const float gate = total(col, 2 * j), up = total(col, 2 * j + 1);
-                        a.h[static_cast<size_t>(plan.order[first + col]) * (a.n / 2) + done * 8 + j] =
-                            __fmul_rn(__fdiv_rn(gate, 1.0f + expf(-gate)), up);
+#pragma unroll
+                for (int k = 0; k < HELD; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // column g: block g of row k (NVFP4), block g % 4 of row 2 k + g / 4 (MXFP4)
+                        const int r = FMT == md::NV ? k : 2 * k + (g >> 2);
+                        const bool mine_too = (FMT == md::NV ? g == 2 * t4 + i : (g & 3) == t4) && r < rows;
+                        b[k][i] = s_rows + static_cast<size_t>(mine_too ? r : rows) * l.pitch + t4 * 16;
+                    }
+            }
+            auto multiply = [&](const md::Piece<FMT>& p) {
+                if constexpr (SETS == 0) md::step_products<FMT>(p, b[0][0], step, t4, a.parts, l.part_bytes, acc);
+                else md::step_blocks<FMT, HELD>(p, b, step, t4, acc);
+            };
+            int whole = -1;
+            auto close = [&](int tl) {
+                const int from = tl * a.steps, to = from + a.steps;
+                const int place = from < run0 ? 0 : (to > run1 ? 1 : 2);
+                if (place == 2) whole = tl;
+                float* d = mine + place * md::SUM_FLOATS + g;
+                if constexpr (SETS == 0) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        d[(2 * t4) * 36 + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2];
+                        d[(2 * t4 + 1) * 36 + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2 + 1];
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < HELD; ++k) {
+                        float v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            v[j] = acc[k * 4 + j];
+                            v[j] += __shfl_xor_sync(0xFFFFFFFFu, v[j], 1);
+                            if (FMT == md::NV) v[j] += __shfl_xor_sync(0xFFFFFFFFu, v[j], 2);
+                        }
+                        if (FMT == md::NV) {             // lane t has row j = t to write, of column k
+                            d[k * 36 + 8 * t4] = t4 == 0 ? v[0] : (t4 == 1 ? v[1] : (t4 == 2 ? v[2] : v[3]));
+                        } else {                         // rows t % 2 * 2 and + 1, of column 2 k + t / 2
+                            float* e = d + (2 * k + (t4 >> 1)) * 36 + 16 * (t4 & 1);
+                            e[0] = t4 & 1 ? v[2] : v[0];
+                            e[8] = t4 & 1 ? v[3] : v[1];
+                        }
                     }
                 }
+                clear();
+            };
+            for (bool met = false;;) {
+                int place = 2, others = warp + 1;          // whose pieces make up the tile that is finished below
+                if (at < run1) {
+#pragma unroll
+                    for (int i = 0; i < F::AHEAD; ++i) {  // a tile has at least MIN_STEPS steps: at most one ends here
+                        if (at < run1) {
+                            fetch(buf[(i + F::AHEAD - 1) % F::AHEAD]);
+                            multiply(buf[i]);
+                            ++at;
+                            const bool ends = ++step == a.steps;
+                            if (ends || at == run1) close(tile);
+                            if (ends) {
+                                step = 0;
+                                ++tile;
+                            }
+                        }
+                    }
+                } else if (!met) {
+                    // every piece is there: the warp whose run has a tile's first step adds them
+                    __syncthreads();
+                    met = true;
+                    const int last = tile - (step == 0 ? 1 : 0), from = last * a.steps, to = from + a.steps;
+                    if (run0 < run1 && from >= run0 && to > run1) {
+                        whole = last;
+                        place = 1;
+                        while (others < WARPS && all * others / WARPS < to) ++others;
+                    }
+                } else {
+                    break;
+                }
+                if (whole < 0) continue;
+                __syncwarp();        // the lanes' sums are there
+                // Scales and the activation of a tile's sums, and the results to memory: a lane is a row.
+                const int tt = tile0 + whole;
+                whole = -1;
+                const int r = md::row_of(tt, lane & 7, lane >> 3);
+                const bool ours = r < a.n && 2 * tt + (lane >> 4) >= unit0 && 2 * tt + (lane >> 4) < unit1;
+                float common = 1.0f;
+                if (FMT == md::F8) common = *reinterpret_cast<const float*>(a.scale);
+                if (FMT == md::NV) common = *a.global_scale;
+                if (FMT == md::I8) common = ours ? __ldg(reinterpret_cast<const float*>(a.scale) + static_cast<size_t>(expert) * a.n + r) : 0.f;
+                for (int c = 0; c < rows; ++c) {
+                    float v = mine[place * md::SUM_FLOATS + c * 36 + lane];
+                    for (int w = warp + 1; w < others; ++w)
+                        if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * md::SUM_FLOATS) + c * 36 + lane];      // (not of an empty run)
+                    v = v * s_inverse[c] * common;
+                    const int entry = plan.order[first + c];
+                    if (DOWN) {
+                        if (ours) a.y[static_cast<size_t>(entry) * a.n + r] = v;
+                    } else {
+                        // rows 2i (gate) and 2i + 1 (up) are neighbouring lanes
+                        const float up = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+                        if (ours && (lane & 1) == 0)
+                            a.h[static_cast<size_t>(entry) * (a.n / 2) + (r >> 1)] = __fmul_rn(__fdiv_rn(v, 1.0f + expf(-v)), up);
+                    }
+                }
+                __syncwarp();        // read, before the warp's next sums
             }
         };
-        // two steps at a time, so that the two sets of registers keep their names
-        while (more) {
-            int tl = tile, st = step;
-            bool next = advance(tl, st);
-            if (next) {
-                const int was = tile;
-                tile = tl;
-                if (tl != was) locate();
-                odd.load(a, row0, row1, sc0, sc1, st, t4);
-                tile = was;
-            }
-            md::step_products<FMT, NT>(even, b, step, nt_used, a.parts, l.part_bytes, acc);
-            if (!next || tl != tile) finish(tile);
-            tile = tl;
-            step = st;
-            if (!next) break;
-            more = advance(tl, st);
-            if (more) {
-                const int was = tile;
-                tile = tl;
-                if (tl != was) locate();
-                even.load(a, row0, row1, sc0, sc1, st, t4);
-                tile = was;
-            }
-            md::step_products<FMT, NT>(odd, b, step, nt_used, a.parts, l.part_bytes, acc);
-            if (!more || tl != tile) finish(tile);
-            tile = tl;
-            step = st;
+        if constexpr (FMT == md::NV) {
+            if (rows == 1) stream(md::Way<1>());
+            else if (rows == 2) stream(md::Way<2>());
+            else stream(md::Way<0>());
+        } else if constexpr (FMT == md::MX) {
+            if (rows <= 2) stream(md::Way<1>());
+            else stream(md::Way<2>());
+        } else {
+            stream(md::Way<0>());
         }
     }
 
@@ -685,32 +816,59 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         }
         // Every result of this CTA is in memory before it counts itself in.
         __threadfence();
+        if (threadIdx.x == 0) s_misc[1] = 0;
         __syncthreads();
-        int* s_last = reinterpret_cast<int*>(s_rows);               // flags of the tiles that this CTA completes
-        const long long mine = end - begin;
-        for (long long i = threadIdx.x; i < a.tiles; i += THREADS) s_last[i] = 0;
-        __syncthreads();
-        for (long long i = threadIdx.x; i < mine; i += THREADS) {
-            const int tile = static_cast<int>((begin + i) % a.tiles);
-            if (atomicAdd(&a.arrived[tile], 1) == plan.segments - 1) s_last[tile] = 1;
+        int* s_list = reinterpret_cast<int*>(s_rows);               // the units that this CTA completes
+        for (int i = begin + threadIdx.x; i < end; i += THREADS) {
+            const int unit = i - md::quotient(i, span, a.div_span) * span - a.entry_cost;
+            if (unit >= 0 && atomicAdd(&a.arrived[unit], 1) == plan.segments - 1) s_list[atomicAdd(&s_misc[1], 1)] = unit;
         }
         __syncthreads();
         __threadfence();
-        // with no entry at all (every logit masked) nobody counts: the CTAs share the zeros
-        const bool none = plan.segments == 0;
-        for (int tile = none ? blockIdx.x : 0; tile < a.tiles; tile += none ? gridDim.x : 1) {
-            if (!none && s_last[tile] == 0) continue;
-            for (int i = threadIdx.x; i < a.tokens * 16; i += THREADS) {
-                const int t = i >> 4, col = tile * 16 + (i & 15);
-                if (col >= a.n) continue;
-                float s = 0.f;
-                for (int j = 0; j < a.k; ++j) {
-                    const int entry = t * a.k + j;
-                    if (plan.ids[entry] >= 0) s = fmaf(plan.weights[entry], __ldcg(a.y + static_cast<size_t>(entry) * a.n + col), s);
+        // With no entry at all (every logit masked) nobody counts: the CTAs share the zeros.  Four columns a thread: half of a
+        // row group of eight.
+        const bool none = plan.segments == 0, vec = a.n % 4 == 0;
+        const int listed = none ? (a.units - bid + ctas - 1) / ctas : s_misc[1];
+        const int each = a.tokens * 4;
+        for (int i = threadIdx.x; i < listed * each; i += THREADS) {
+            const int which = i / each, in = i - which * each, t = in >> 2;
+            const int unit = none ? bid + which * ctas : s_list[which];
+            const int col = md::row_of(unit >> 1, (in & 1) * 4, (unit & 1) * 2 + (in >> 1 & 1));
+            if (col >= a.n) continue;
+            const float* y = a.y + static_cast<size_t>(t) * a.k * a.n + col;
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int j0 = 0; j0 < a.k; j0 += 8) {         // eight slots' loads in flight
+                float4 u[8];
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool in = j0 + j < a.k && plan.ids[t * a.k + j0 + j] >= 0;
+                    const float* q = y + static_cast<size_t>(j0 + j) * a.n;
+                    p[j] = in ? plan.weights[t * a.k + j0 + j] : 0.f;
+                    u[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (in && vec) {
+                        u[j] = __ldcg(reinterpret_cast<const float4*>(q));
+                    } else if (in) {
+                        u[j].x = __ldcg(q);
+                        if (col + 1 < a.n) u[j].y = __ldcg(q + 1);
+                        if (col + 2 < a.n) u[j].z = __ldcg(q + 2);
+                        if (col + 3 < a.n) u[j].w = __ldcg(q + 3);
+                    }
                 }
-                const size_t at = static_cast<size_t>(t) * a.n + col;
-                if (a.out_dtype == DSL_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(s);
-                else static_cast<float*>(a.out)[at] = s;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    s[0] = fmaf(p[j], u[j].x, s[0]);
+                    s[1] = fmaf(p[j], u[j].y, s[1]);
+                    s[2] = fmaf(p[j], u[j].z, s[2]);
+                    s[3] = fmaf(p[j], u[j].w, s[3]);
+                }
+            }
+            const size_t to = static_cast<size_t>(t) * a.n + col;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (col + c >= a.n) break;
+                if (a.out_dtype == DSL_BF16) static_cast<__nv_bfloat16*>(a.out)[to + c] = __float2bfloat16_rn(s[c]);
+                else static_cast<float*>(a.out)[to + c] = s[c];
             }
         }
     }
@@ -721,48 +879,43 @@ namespace md {
 
 constexpr int SMEM_LIMIT = 227 * 1024;
 
-// Rows an expert's CTA may hold, K cut and shared memory; false when not even one row fits.
-static bool plan_launch(Args& a, int elems, int nt, int sms, int* smem_bytes) {
-    a.tiles = (a.n + 15) / 16;
+// Rows of an expert that a CTA may hold, and its shared memory; false when not even one row fits.
+static bool plan_launch(Args& a, int format, int* smem_bytes) {
+    a.units = (a.n + 127) / 128 * 8;
     a.steps = (a.row_bytes + STEP - 1) / STEP;
-    a.block_rows = 1;
-    const int most = a.tokens < nt * 8 ? a.tokens : nt * 8;
+    if (a.steps < MIN_STEPS) a.steps = MIN_STEPS;
+    static const int forced = [] { const char* e = getenv("DSLGEMM_MOE_COST"); return e != nullptr ? atoi(e) : -1; }();
+    a.entry_cost = (forced >= 0 ? forced : 7000) / a.row_bytes;
+    const auto inverse = [](int d) { return static_cast<unsigned>(0xFFFFFFFFull / static_cast<unsigned>(d)); };
+    a.div_span = inverse(a.units + a.entry_cost);
+    a.div_steps = inverse(a.steps);
+    a.div_k = inverse(a.k);
+    const bool fp4 = format == DSL_W_NVFP4 || format == DSL_W_MXFP4;
+    const int elems = fp4 ? 32 : (format == DSL_W_BF16 ? 8 : 16);
+    const int cap = format == DSL_W_MXFP4 ? Fmt<MX>::ROWS : Fmt<NV>::ROWS, most = a.tokens < cap ? a.tokens : cap;
+    int fits = 0;
     for (int r = 1; r <= most; ++r) {
-        Args t = a;
-        t.block_rows = r;
-        const Layout l = layout_of(t, elems, nt);
-        if (l.total > SMEM_LIMIT) {
-            if (r == 1) return false;
-            break;
-        }
         a.block_rows = r;
+        const Layout l = layout_of(a, elems, fp4);
+        if (l.total > SMEM_LIMIT) break;
         *smem_bytes = l.total;
+        fits = r;
     }
-    // flags of the finished tiles share the rows' region
-    const int flags = layout_of(a, elems, nt).rows + a.tiles * 4;
-    if (flags > SMEM_LIMIT) return false;
-    if (flags > *smem_bytes) *smem_bytes = flags;
-    // Warps on one tile: enough of them that each of a CTA's groups has about four tiles to run through, never more than steps.
-    // Tiles a CTA: of the experts that `tokens` random choices reach on average.
-    double miss = 1.0;
-    for (int i = 0; i < a.tokens; ++i) miss *= 1.0 - static_cast<double>(a.k) / a.experts;
-    const double per_cta = a.experts * (1.0 - miss) * a.tiles / sms;
-    int split = 1;
-    while (split < WARPS && split * 2 <= a.steps && per_cta * split < 4.0 * WARPS) split *= 2;
-    a.split = split;
-    return true;
+    a.block_rows = fits;
+    return fits > 0;
 }
 
-template <int FMT, int NT, bool DOWN>
-static int launch_one(const Args& a, int smem_bytes, int sms, cudaStream_t st) {
+template <int FMT, bool DOWN>
+static int launch_one(Args& a, int smem_bytes, int sms, cudaStream_t st) {
     static PerDeviceInt attr_set;   // per device; idempotent, a race here only repeats the same call
     const int dev = current_device_slot();
     if (dev < 0) return static_cast<int>(cudaErrorInvalidDevice);
     if (attr_set.v[dev].load(std::memory_order_acquire) == 0) {
-        const cudaError_t e = cudaFuncSetAttribute(moe_decode_kernel<FMT, NT, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+        const cudaError_t e = cudaFuncSetAttribute(moe_decode_kernel<FMT, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
         if (e != cudaSuccess) return static_cast<int>(e);
         attr_set.v[dev].store(1, std::memory_order_release);
     }
+    a.div_grid = 0xFFFFFFFFu / static_cast<unsigned>(sms);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(sms));
     cfg.blockDim = dim3(THREADS);
@@ -773,7 +926,7 @@ static int launch_one(const Args& a, int smem_bytes, int sms, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, moe_decode_kernel<FMT, NT, DOWN>, a));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, moe_decode_kernel<FMT, DOWN>, a));
 }
 
 static Args side(const dsl_weight* w, int tokens, int k, int x_dtype) {
@@ -795,18 +948,14 @@ static Args side(const dsl_weight* w, int tokens, int k, int x_dtype) {
 }
 
 template <int FMT>
-static int launch_fmt(Args& up, Args& down, int sms, cudaStream_t st) {
-    const int nt = up.tokens > 8 ? 2 : 1;
+static int launch_fmt(int format, Args& up, Args& down, int sms, cudaStream_t st) {
     int bytes_up = 0, bytes_down = 0;
-    if (!plan_launch(up, Fmt<FMT>::ELEMS, nt, sms, &bytes_up) || !plan_launch(down, Fmt<FMT>::ELEMS, nt, sms, &bytes_down))
+    if (!plan_launch(up, format, &bytes_up) || !plan_launch(down, format, &bytes_down))
         return DSL_ERR_TOO_LARGE;
-    up.arrived_count = down.tiles;
-    int rc = nt == 1 ? launch_one<FMT, 1, false>(up, bytes_up, sms, st) : launch_one<FMT, 2, false>(up, bytes_up, sms, st);
-    if (rc != 0) return rc;
-    return nt == 1 ? launch_one<FMT, 1, true>(down, bytes_down, sms, st) : launch_one<FMT, 2, true>(down, bytes_down, sms, st);
+    up.arrived_count = down.units;
+    const int rc = launch_one<FMT, false>(up, bytes_up, sms, st);
+    return rc != 0 ? rc : launch_one<FMT, true>(down, bytes_down, sms, st);
 }
-
-static int elems_of(int format) { return format == DSL_W_NVFP4 || format == DSL_W_MXFP4 ? 32 : (format == DSL_W_BF16 ? 8 : 16); }
 
 // What the entry point takes; 0 or DSL_ERR_*.
 static int check(const dsl_weight* gu, const dsl_weight* dn, int tokens, int k, int x_dtype) {
@@ -821,13 +970,13 @@ static int check(const dsl_weight* gu, const dsl_weight* dn, int tokens, int k, 
     if (gu->k % multiple != 0 || dn->k % multiple != 0) return DSL_ERR_SHAPE;
     if (tokens < 0 || k < 1 || k > 32 || k > gu->groups) return DSL_ERR_SHAPE;
     if (tokens > DSL_MOE_DECODE_MAX_TOKENS) return DSL_ERR_TOO_LARGE;
-    // rows that a CTA cannot hold, or sizes that 32-bit offsets inside a row or a tile table could not take
-    if (gu->k > (1 << 20) || dn->k > (1 << 20) || dn->n > (1 << 20)) return DSL_ERR_TOO_LARGE;
+    // sizes whose products the kernels form in 32 bits: 96 rows of a weight, units and steps of all segments
+    if (gu->k > (1 << 20) || dn->k > (1 << 20) || dn->n > (1 << 18)) return DSL_ERR_TOO_LARGE;
     if (tokens > 0) {
         int bytes;
         for (int i = 0; i < 2; ++i) {
             Args a = side(i == 0 ? gu : dn, tokens, k, i == 0 ? x_dtype : DSL_F32);
-            if (!plan_launch(a, elems_of(gu->format), tokens > 8 ? 2 : 1, 148, &bytes)) return DSL_ERR_TOO_LARGE;
+            if (!plan_launch(a, gu->format, &bytes)) return DSL_ERR_TOO_LARGE;
         }
     }
     return 0;
@@ -843,7 +992,7 @@ using namespace dsl;
 extern "C" size_t dsl_moe_decode_scratch_bytes(const dsl_weight* gate_up, const dsl_weight* down, int tokens, int k, int x_dtype) {
     if (md::check(gate_up, down, tokens, k, x_dtype) != 0 || tokens == 0) return 0;
     const size_t entries = static_cast<size_t>(tokens) * k;
-    return md::up256(entries * down->k * 4) + md::up256(entries * down->n * 4) + md::up256((down->n + 15) / 16 * 4ull);
+    return md::up256(entries * down->k * 4) + md::up256(entries * down->n * 4) + md::up256((down->n + 127) / 128 * 8 * 4ull);
 }
 
 extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, int logits_dtype, int tokens, int k, int renorm,
@@ -884,11 +1033,11 @@ extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, in
     const int sms = sm_count();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (format) {
-        case DSL_W_FP8: return md::launch_fmt<md::F8>(up, dn, sms, st);
-        case DSL_W_FP8_BLOCK128: return md::launch_fmt<md::F8G>(up, dn, sms, st);
-        case DSL_W_INT8: return md::launch_fmt<md::I8>(up, dn, sms, st);
-        case DSL_W_NVFP4: return md::launch_fmt<md::NV>(up, dn, sms, st);
-        case DSL_W_MXFP4: return md::launch_fmt<md::MX>(up, dn, sms, st);
-        default: return md::launch_fmt<md::BF>(up, dn, sms, st);
+        case DSL_W_FP8: return md::launch_fmt<md::F8>(format, up, dn, sms, st);
+        case DSL_W_FP8_BLOCK128: return md::launch_fmt<md::F8G>(format, up, dn, sms, st);
+        case DSL_W_INT8: return md::launch_fmt<md::I8>(format, up, dn, sms, st);
+        case DSL_W_NVFP4: return md::launch_fmt<md::NV>(format, up, dn, sms, st);
+        case DSL_W_MXFP4: return md::launch_fmt<md::MX>(format, up, dn, sms, st);
+        default: return md::launch_fmt<md::BF>(format, up, dn, sms, st);
     }
 }
