@@ -14,8 +14,8 @@
 //   * A CTA's steps, tile after tile, are dealt to its 16 warps in equal runs.  A tile that lies inside a run is finished by its
 //     warp; the pieces of the others meet in shared memory after the last step and are added in order.
 //   * The rows of x (or h) that the current expert multiplies are kept in shared memory, as 16-bit values in the order in which the
-//     tensor core's B fragments want them.  Weights go from global memory straight into registers (two or three steps of four
-//     16-byte loads a lane in flight while another is multiplied: 64 or 96 KB an SM), are widened there to f16 or bf16, exactly, and meet the
+//     tensor core's B fragments want them.  Weights go from global memory straight into registers (two steps of four 16-byte
+//     loads a lane in flight while a third is multiplied: 64 KB an SM; three gained nothing), are widened there to f16 or bf16, exactly, and meet the
 //     rows in mma.sync m16n8k16 with fp32 sums.  The order of K inside a step is free as long as both sides agree: lane (g, t) of
 //     a warp holds 16 consecutive bytes of its four rows, every load covers whole 64-byte pieces, and no weight passes through
 //     shared memory.  (tcgen05 would want the widened weight written to shared memory first, for tiles of which at most one column
@@ -30,11 +30,14 @@
 // largest one.  An fp32 x and the hidden activation round to 11 bits (f16), or to 16 (two bf16 terms) with bf16 weights - more than
 // the 8 bits of the bf16 hidden activation that the layer of quantised GEMMs passes on.  All sums are fp32.
 //
-// Layer of 64 experts, top 8, K = D = 4096, H = 1536:
+// Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us (share of the rate at which the chosen experts' bytes can be
+// copied): one token NVFP4 35 (37 %), FP8 40 (57 %); 8 tokens NVFP4 114 (62 %), FP8 128x128 154 (81 %); 16 tokens NVFP4 161 (58 %).
+// 8 experts, top 2, H = 14336, 3 tokens BF16 333 (75 %).  What is left: about 15 us of a layer in which nothing streams (routing and
+// list 3.5 us and the first rows 1.5 us of either kernel, the last sums and counters), and, in FP4, CTAs that wait for the one
+// whose expert has more rows.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
-#include <stdlib.h>
 
 #include <atomic>
 
@@ -49,6 +52,7 @@ constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int SUM_FLOATS = 8 * 36;       // a tile's sums: eight columns of 32 rows, 36 apart (no bank conflicts)
 constexpr int STEP = 64;                 // bytes of a weight row that a warp takes at once
+constexpr int AHEAD = 3;                 // steps that a lane has registers for: all but one in flight
 constexpr int MIN_STEPS = 4;             // of a tile (short rows: steps without bytes)
 
 enum { F8 = 0, F8G = 1, I8 = 2, NV = 3, MX = 4, BF = 5 };
@@ -59,7 +63,6 @@ struct Fmt {
     static constexpr bool BF16 = FMT == BF;                                              // type of the products
     static constexpr int PARTS = FMT == BF ? 2 : 1;                                      // 16-bit terms of an activation, at most
     static constexpr bool FP4 = FMT == NV || FMT == MX;
-    static constexpr int AHEAD = FP4 ? 3 : 4;            // steps that a lane has registers for: all but one in flight
     static constexpr int ROWS = FMT == MX ? 4 : 8;       // activation rows that a CTA multiplies at a time, at most
 };
 
@@ -73,9 +76,9 @@ struct Args {
     const float* global_scale;
     int n, kdim, row_bytes, katoms;
     int units;                   // of 16 rows: 8 for every 128, the last ones possibly without rows
-    int entry_cost;              // what starting on an expert costs a CTA, in units
+    int entry_cost;              // what starting on an expert costs a CTA, in eighths of a unit against one row
     int steps;                   // of a tile
-    unsigned div_span, div_steps, div_grid, div_k;      // 2^32 / (units + entry_cost), / steps, / CTAs, / k: see quotient()
+    unsigned div_steps, div_grid, div_k;      // 2^32 / steps, / CTAs, / k: see quotient()
     int block_rows;              // rows of one expert that a CTA holds at a time
     int parts;                   // 16-bit terms an activation (2 only with bf16 products)
     float* h;                    // up: [entries, n / 2]
@@ -101,6 +104,7 @@ struct Plan {
     int* seg_expert;   // [segments]: an expert with at most block_rows of its rows
     int* seg_first;    //             first place in `order`
     int* seg_rows;
+    int* seg_start;    //             first place in the list of work; [segments] its end
     uint32_t* tokens;  // [experts] who chose it, a bit each
     int* base;         // [experts] its first place in `order`
     int segments;
@@ -187,8 +191,22 @@ __device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, c
     }
 }
 
-// All threads.  `work`: WARPS * experts words that nothing else uses yet.
-__device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work, int* s_segments) {
+// Cost of a unit, in eighths, against so many rows.  Measured a unit, us: NVFP4 1 / 2 / 3 rows 0.89 / 1.06 / 1.06 (K = 4096), MXFP4
+// 1 / 2 / 3 / 4 rows 0.67 / 0.67 / 0.87 / 0.86 (K = 2912), FP8 128x128 1.31 whatever the rows.  In the shares: 8 tokens NVFP4 142 ->
+// 123 us a layer, 16 tokens MXFP4 196 -> 172.
+template <int FMT>
+__device__ __forceinline__ int unit_cost(int rows) { return FMT == NV ? (rows == 1 ? 8 : 9) : (FMT == MX && rows > 2 ? 10 : 8); }
+// Units that `cost` pays for.
+template <int FMT>
+__device__ __forceinline__ int units_for(int cost, int rows) {
+    const int each = unit_cost<FMT>(rows);
+    return cost <= 0 ? 0 : (each == 8 ? cost >> 3 : (each == 9 ? cost / 9 : cost / 10));
+}
+
+// All threads.  `work`: WARPS * experts words that nothing else uses yet.  [begin, end): this CTA's share of the list of work, which
+// starts in segment `seg`.
+template <int FMT>
+__device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work, int* s_misc, int& begin, int& end, int& seg) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int e = threadIdx.x; e < a.experts; e += THREADS) p.tokens[e] = 0u;
     __syncthreads();
@@ -199,16 +217,22 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work
     __syncthreads();
     if (warp == 0) {
         // experts 32 at a time: their places and segments
-        int rows = 0, segments = 0;
+        int rows = 0, segments = 0, start = 0;
         for (int e0 = 0; e0 < a.experts; e0 += 32) {
             const int e = e0 + lane;
             const int c = e < a.experts ? __popc(p.tokens[e]) : 0;
             const int b = (c + a.block_rows - 1) / a.block_rows;
             int run = c | (b << 16);                           // both sums at once: at most 1024 each
+            const int full = a.entry_cost + a.units * unit_cost<FMT>(a.block_rows), rest = c - (b - 1) * a.block_rows;
+            const int cost = b > 0 ? (b - 1) * full + a.entry_cost + a.units * unit_cost<FMT>(rest) : 0;
+            int run_cost = cost;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
-                if (lane >= o) run += v;
+                const int v = __shfl_up_sync(0xFFFFFFFFu, run, o), vc = __shfl_up_sync(0xFFFFFFFFu, run_cost, o);
+                if (lane >= o) {
+                    run += v;
+                    run_cost += vc;
+                }
             }
             const int first = rows + (run & 0xFFFF) - c, s0 = segments + (run >> 16) - b;
             if (c > 0) p.base[e] = first;
@@ -216,20 +240,32 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work
                 p.seg_expert[s0 + i] = e;
                 p.seg_first[s0 + i] = first + i * a.block_rows;
                 p.seg_rows[s0 + i] = min(a.block_rows, c - i * a.block_rows);
+                p.seg_start[s0 + i] = start + run_cost - cost + i * full;
             }
             run = __shfl_sync(0xFFFFFFFFu, run, 31);
             rows += run & 0xFFFF;
             segments += run >> 16;
+            start += __shfl_sync(0xFFFFFFFFu, run_cost, 31);
         }
-        if (lane == 0) *s_segments = segments;
+        if (lane == 0) {
+            s_misc[0] = segments;
+            p.seg_start[segments] = start;
+        }
     }
     __syncthreads();
     for (int t = warp; t < a.tokens; t += WARPS) {
         const int e = lane < a.k ? p.ids[t * a.k + lane] : -1;
         if (e >= 0) p.order[p.base[e] + __popc(p.tokens[e] & ((1u << t) - 1u))] = t * a.k + lane;
     }
+    p.segments = s_misc[0];
+    const int places = p.seg_start[p.segments], ctas = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
+    const int share = quotient(places, ctas, a.div_grid), more_than = places - share * ctas;
+    begin = bid * share + min(bid, more_than);
+    end = begin + share + (bid < more_than ? 1 : 0);
+    for (int i = threadIdx.x; i < p.segments; i += THREADS)
+        if (p.seg_start[i] <= begin && begin < p.seg_start[i + 1]) s_misc[2] = i;
     __syncthreads();
-    p.segments = *s_segments;
+    seg = s_misc[2];
 }
 
 // ---- 16-bit products ---------------------------------------------------------------------------------------------------------------
@@ -269,13 +305,21 @@ __device__ __forceinline__ uint32_t widen_int8(uint32_t biased, uint32_t selecto
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// 16 bytes that are read once.  Where streaming bounds (all but the FP4 formats) the L2 is asked for 256 bytes of the row, which the
+// warp comes to in its next steps: the memory reads longer pieces (8 tokens FP8 171 -> 157 us a layer, 3 tokens BF16 390 -> 331).
+template <int FMT>
 __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
+    uint4 r;
+    if (Fmt<FMT>::FP4) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    else asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+// Scale bytes: past the L1 too, which the lines of a whole atom would run through (8 tokens NVFP4 124 -> 114 us a layer).
+__device__ __forceinline__ uint4 load_table(const uint8_t* p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
-
-__device__ __forceinline__ uint4 load_table(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : (j == 1 ? v.y : (j == 2 ? v.z : v.w)); }
 
 // What a lane holds of one step: 16 bytes of each of its four rows (g + 32 j of the tile), with the scales.
@@ -293,7 +337,7 @@ struct Piece {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             w[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (in && (rows >> j & 1u)) w[j] = load_stream(row + static_cast<size_t>(static_cast<unsigned>(j * pitch)) + at);
+            if (in && (rows >> j & 1u)) w[j] = load_stream<FMT>(row + static_cast<size_t>(static_cast<unsigned>(j * pitch)) + at);
         }
         // NV: two blocks a piece, so atom piece / 2; MX: one, atom piece / 4, which all lanes of a quad need for its maximum
         if (FMT == NV) s = in ? load_table(scale + static_cast<size_t>(at >> 5) * 512) : make_uint4(0u, 0u, 0u, 0u);
@@ -545,7 +589,7 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
 
 // ---- shared memory ----------------------------------------------------------------------------------------------------------------
 struct Layout {
-    int ids, weights, order, seg_expert, seg_first, seg_rows, chosen, base, misc, sums, rows, total;
+    int ids, weights, order, seg_expert, seg_first, seg_rows, seg_start, chosen, base, misc, sums, rows, total;
     int pitch, part_bytes;
 };
 // `elems`: elements of a weight in 16 bytes; the rows' region doubles as the router's room and the list of finished units.
@@ -560,9 +604,10 @@ __host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) 
     l.seg_expert = take(entries * 4);
     l.seg_first = take(entries * 4);
     l.seg_rows = take(entries * 4);
+    l.seg_start = take((entries + 1) * 4);
     l.chosen = take(a.experts * 4);
     l.base = take(a.experts * 4);
-    l.misc = take(16 + 2 * 8 * 4);                                     // two counters; amax of the rows, their inverse factors
+    l.misc = take(16 + 2 * 8 * 4);                                     // three counters; amax of the rows, their inverse factors
     l.sums = take(3 * WARPS * SUM_FLOATS * 4);                         // a run's first piece of a tile, its last one, a whole one
     l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 128
     l.pitch = l.part_bytes * a.parts + 64;                             // two rows start half a bank round apart
@@ -595,9 +640,10 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     plan.seg_expert = reinterpret_cast<int*>(smem + l.seg_expert);
     plan.seg_first = reinterpret_cast<int*>(smem + l.seg_first);
     plan.seg_rows = reinterpret_cast<int*>(smem + l.seg_rows);
+    plan.seg_start = reinterpret_cast<int*>(smem + l.seg_start);
     plan.tokens = reinterpret_cast<uint32_t*>(smem + l.chosen);
     plan.base = reinterpret_cast<int*>(smem + l.base);
-    int* s_misc = reinterpret_cast<int*>(smem + l.misc);               // [0] segments, [1] units that this CTA completes
+    int* s_misc = reinterpret_cast<int*>(smem + l.misc);               // [0] segments, [1] units that this CTA completes, [2] its first segment
     uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + l.misc + 16);
     float* s_inverse = reinterpret_cast<float*>(smem + l.misc + 16 + 32);
     float* s_sums = reinterpret_cast<float*>(smem + l.sums);
@@ -615,20 +661,21 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     // f16 rows are what they are, bf16 ones as bf16 too; the second bf16 term of an fp32 value wants room below the first
     const bool scaled = DOWN || a.x_dtype == DSL_F32 || (a.x_dtype == DSL_BF16 && !F::BF16);
     // Down may get this far while up still runs: logits and weights were complete before up started.
-    md::make_plan(a, plan, reinterpret_cast<uint32_t*>(s_rows), s_misc);
     // The list of work: every expert's units behind entry_cost places without work, so that a CTA which passes from one expert to
     // the next, and has to fetch that one's rows, is dealt less.
-    const int span = a.units + a.entry_cost, items = plan.segments * span;
+    int begin, end, seg0;
+    md::make_plan<FMT>(a, plan, reinterpret_cast<uint32_t*>(s_rows), s_misc, begin, end, seg0);
     const int ctas = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
-    const int share = md::quotient(items, ctas, a.div_grid), more_than = items - share * ctas;
-    const int begin = bid * share + min(bid, more_than), end = begin + share + (bid < more_than ? 1 : 0);
     bool waited = !DOWN;
+    auto units_of = [&](int seg, int& unit0, int& unit1) {
+        const int start = plan.seg_start[seg], rows = plan.seg_rows[seg];
+        unit0 = md::units_for<FMT>(max(begin, start) - start - a.entry_cost, rows);
+        unit1 = md::units_for<FMT>(min(end, plan.seg_start[seg + 1]) - start - a.entry_cost, rows);
+    };
 
-    for (int item = begin; item < end;) {
-        const int seg = md::quotient(item, span, a.div_span);
-        const int off0 = item - seg * span, off1 = min(span, off0 + (end - item));
-        item += off1 - off0;
-        const int unit0 = max(0, off0 - a.entry_cost), unit1 = max(0, off1 - a.entry_cost);
+    for (int seg = seg0; begin < end && seg < plan.segments && plan.seg_start[seg] < end; ++seg) {
+        int unit0, unit1;
+        units_of(seg, unit0, unit1);
         if (unit0 == unit1) continue;
         const int expert = plan.seg_expert[seg], first = plan.seg_first[seg], rows = plan.seg_rows[seg];
         // this CTA's tiles of the expert, and this warp's run of their steps
@@ -638,7 +685,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         int at = run0, tile = md::quotient(run0, a.steps, a.div_steps), step = run0 - tile * a.steps;      // tile counts from tile0
 
         // Where the loads are: up to AHEAD - 1 steps before the products.
-        static_assert(F::AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
+        static_assert(md::AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
         const int pitch = 32 * a.row_bytes;
         int l_at = run0, l_step = step, l_tile = tile0 + tile;
         const uint8_t *l_row = nullptr, *l_scale = nullptr;
@@ -652,7 +699,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
             if (FMT == md::NV || FMT == md::MX) l_scale = a.scale + block * a.katoms * 512 + ((l_tile & 3) * 8 + g) * 16;
             if (FMT == md::F8G) l_scale = a.scale + block * (a.kdim / 128) * 4;
         };
-        md::Piece<FMT> buf[F::AHEAD];
+        md::Piece<FMT> buf[md::AHEAD];
         auto fetch = [&](md::Piece<FMT>& p) {
             if (l_at < run1) {
                 p.load(a, l_row, pitch, l_rows, l_scale, l_step, t4);
@@ -666,7 +713,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         };
         if (run0 < run1) locate();
 #pragma unroll
-        for (int i = 0; i + 1 < F::AHEAD; ++i) fetch(buf[i]);
+        for (int i = 0; i + 1 < md::AHEAD; ++i) fetch(buf[i]);
         if (!waited) {           // the hidden activation is up's
             griddep_wait();
             griddep_launch_dependents();
@@ -742,9 +789,9 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 int place = 2, others = warp + 1;          // whose pieces make up the tile that is finished below
                 if (at < run1) {
 #pragma unroll
-                    for (int i = 0; i < F::AHEAD; ++i) {  // a tile has at least MIN_STEPS steps: at most one ends here
+                    for (int i = 0; i < md::AHEAD; ++i) {  // a tile has at least MIN_STEPS steps: at most one ends here
                         if (at < run1) {
-                            fetch(buf[(i + F::AHEAD - 1) % F::AHEAD]);
+                            fetch(buf[(i + md::AHEAD - 1) % md::AHEAD]);
                             multiply(buf[i]);
                             ++at;
                             const bool ends = ++step == a.steps;
@@ -799,7 +846,6 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         };
         if constexpr (FMT == md::NV) {
             if (rows == 1) stream(md::Way<1>());
-            else if (rows == 2) stream(md::Way<2>());
             else stream(md::Way<0>());
         } else if constexpr (FMT == md::MX) {
             if (rows <= 2) stream(md::Way<1>());
@@ -819,9 +865,11 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         if (threadIdx.x == 0) s_misc[1] = 0;
         __syncthreads();
         int* s_list = reinterpret_cast<int*>(s_rows);               // the units that this CTA completes
-        for (int i = begin + threadIdx.x; i < end; i += THREADS) {
-            const int unit = i - md::quotient(i, span, a.div_span) * span - a.entry_cost;
-            if (unit >= 0 && atomicAdd(&a.arrived[unit], 1) == plan.segments - 1) s_list[atomicAdd(&s_misc[1], 1)] = unit;
+        for (int seg = seg0; begin < end && seg < plan.segments && plan.seg_start[seg] < end; ++seg) {
+            int unit0, unit1;
+            units_of(seg, unit0, unit1);
+            for (int unit = unit0 + threadIdx.x; unit < unit1; unit += THREADS)
+                if (atomicAdd(&a.arrived[unit], 1) == plan.segments - 1) s_list[atomicAdd(&s_misc[1], 1)] = unit;
         }
         __syncthreads();
         __threadfence();
@@ -884,10 +932,11 @@ static bool plan_launch(Args& a, int format, int* smem_bytes) {
     a.units = (a.n + 127) / 128 * 8;
     a.steps = (a.row_bytes + STEP - 1) / STEP;
     if (a.steps < MIN_STEPS) a.steps = MIN_STEPS;
-    static const int forced = [] { const char* e = getenv("DSLGEMM_MOE_COST"); return e != nullptr ? atoi(e) : -1; }();
-    a.entry_cost = (forced >= 0 ? forced : 7000) / a.row_bytes;
+    // Starting on an expert (its rows fetched, the pipeline filled and drained) costs a CTA about what 110 KB of weight take it;
+    // one token NVFP4 / FP8 47 / 47 us without that in the shares, 43 / 45 with, 42 / 43 with twice as much, but 16 tokens MXFP4
+    // 253 / 264 with once / twice.
+    a.entry_cost = 8 * 7000 / a.row_bytes;
     const auto inverse = [](int d) { return static_cast<unsigned>(0xFFFFFFFFull / static_cast<unsigned>(d)); };
-    a.div_span = inverse(a.units + a.entry_cost);
     a.div_steps = inverse(a.steps);
     a.div_k = inverse(a.k);
     const bool fp4 = format == DSL_W_NVFP4 || format == DSL_W_MXFP4;
