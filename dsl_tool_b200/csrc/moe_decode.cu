@@ -19,8 +19,7 @@
 //     rows in mma.sync m16n8k16 with fp32 sums.  The order of K inside a step is free as long as both sides agree: lane (g, t) of
 //     a warp holds 16 consecutive bytes of its four rows, every load covers whole 64-byte pieces, and no weight passes through
 //     shared memory.  (tcgen05 would want the widened weight written to shared memory first, for tiles of which at most one column
-//     in eight is used.  The widening - two instructions for two FP4 weights - and not the products' rate is what the FP4 formats
-//     are bound by: an SM widens 64 pairs a clock, and HBM brings 23.)
+//     in eight is used.  The products and the widening are not what bounds: with either left out a layer took as long.)
 //   * Down's results go to scratch by (token, slot); the CTA that delivers a unit's last one adds the slots and writes the output.
 //     Which CTA that is changes nothing: it adds in slot order.
 //
