@@ -110,9 +110,21 @@ __device__ __forceinline__ void store_chunk32_t(const GemmArgs& args, int row, i
     scale32(args, v, s1, s2, rs, f);
     if (args.col_scale != nullptr) {
         const float* cs = args.col_scale + static_cast<size_t>(group) * args.n;
+        if (FULL && col0 + 32 <= args.n && (reinterpret_cast<uintptr_t>(cs + col0) & 15u) == 0) {
+            const float4* c4 = reinterpret_cast<const float4*>(cs + col0);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (col0 + i < args.n) f[i] = __fmul_rn(f[i], cs[col0 + i]);
+            for (int i = 0; i < 8; ++i) {
+                const float4 c = __ldg(c4 + i);
+                f[4 * i] = __fmul_rn(f[4 * i], c.x);
+                f[4 * i + 1] = __fmul_rn(f[4 * i + 1], c.y);
+                f[4 * i + 2] = __fmul_rn(f[4 * i + 2], c.z);
+                f[4 * i + 3] = __fmul_rn(f[4 * i + 3], c.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (col0 + i < args.n) f[i] = __fmul_rn(f[i], cs[col0 + i]);
+        }
     }
     if (FULL && args.act != DSL_ACT_NONE) {
         // columns (2j, 2j+1) = (gate_j, up_j) -> output column col0/2 + j of an [m, n/2] result
@@ -235,6 +247,44 @@ __device__ __forceinline__ void store_chunk32_bf16_warp(const GemmArgs& args, ui
             *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(args.c) + static_cast<size_t>(row) * args.ldc + col0 + 8 * p) = d;
     }
     __syncwarp();
+}
+
+// Plain fp32 result, stored by the whole warp the same way, 16 columns (64 bytes of a row) at a time; the column scales meet the
+// values behind the exchange, where a lane has four neighbouring columns of several rows and loads them once.  Against a lane
+// storing its own row and fetching all 32 scales, 4096 x 4096 x 14336 int8 with both scales: 225 -> 165 us.
+__device__ __forceinline__ void store_chunk32_f32_warp(const GemmArgs& args, uint8_t* scratch, int row_base, int row_end, int col0,
+                                                       int group, const uint32_t (&v)[32], float s1, float s2, float rs, int lane) {
+    float f[32];
+    scale32(args, v, s1, s2, rs, f);
+    const int swz = (lane >> 1) & 3, p = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(scratch + lane * 64 + 16 * (i ^ swz)) =
+                make_float4(f[16 * h + 4 * i], f[16 * h + 4 * i + 1], f[16 * h + 4 * i + 2], f[16 * h + 4 * i + 3]);
+        __syncwarp();
+        const int col = col0 + 16 * h + 4 * p;
+        float4 cs = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (args.col_scale != nullptr) {
+            const float* c = args.col_scale + static_cast<size_t>(group) * args.n + col;
+            cs = make_float4(__ldg(c), __ldg(c + 1), __ldg(c + 2), __ldg(c + 3));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rr = (lane >> 2) + 8 * i;
+            float4 d = *reinterpret_cast<const float4*>(scratch + rr * 64 + 16 * (p ^ ((rr >> 1) & 3)));
+            if (args.col_scale != nullptr) {
+                d.x = __fmul_rn(d.x, cs.x);
+                d.y = __fmul_rn(d.y, cs.y);
+                d.z = __fmul_rn(d.z, cs.z);
+                d.w = __fmul_rn(d.w, cs.w);
+            }
+            const int row = row_base + rr;
+            if (row < row_end) *reinterpret_cast<float4*>(static_cast<float*>(args.c) + static_cast<size_t>(row) * args.ldc + col) = d;
+        }
+        __syncwarp();
+    }
 }
 
 }  // namespace dsl

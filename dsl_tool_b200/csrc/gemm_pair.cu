@@ -342,9 +342,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         float s2 = args.s2_dev != nullptr ? *args.s2_dev : args.s2;
         if (args.scale_product) { s1 = s1 * s2; s2 = 1.0f; }
         const bool vec_ok = args.out_bf16 ? (args.ldc % 8 == 0) : (args.ldc % 4 == 0);
-        // plain bf16 results leave through the warp-wide store (rows exchanged in shared memory)
-        const bool warp_store = !SPLIT && args.out_bf16 && vec_ok && args.act == DSL_ACT_NONE && args.out_sf == nullptr;
         uint8_t* epi_scratch = smem + C::OFF_EPI + (warp - 2) * 2048;
+        // plain results leave through the warp-wide stores (rows exchanged in shared memory)
+        const bool warp_store = !SPLIT && vec_ok && args.act == DSL_ACT_NONE && args.out_sf == nullptr;
+        auto store_warp = [&](int row_warp, int row_end, int col0, int group, const uint32_t (&v)[32], float rs) {
+            if (args.out_bf16) store_chunk32_bf16_warp(args, epi_scratch, row_warp, row_end, col0, group, v, s1, s2, rs, lane);
+            else store_chunk32_f32_warp(args, epi_scratch, row_warp, row_end, col0, group, v, s1, s2, rs, lane);
+        };
         bool ok = true;
         long long iter = 0;
         for (long long t = pair_id; t < total_items && ok; t += num_pairs, ++iter) {
@@ -384,7 +388,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 if constexpr (SPLIT)
                     store_partial32(args, ks, row, ti.n0 + ca * 32, row_ok, va);
                 else if (warp_store && ti.n0 + ca * 32 + 32 <= args.n)
-                    store_chunk32_bf16_warp(args, epi_scratch, row_warp, ti.row_end, ti.n0 + ca * 32, ti.group, va, s1, s2, rs, lane);
+                    store_warp(row_warp, ti.row_end, ti.n0 + ca * 32, ti.group, va, rs);
                 else if (row_ok && ti.n0 + ca * 32 < args.n)
                     store_chunk32(args, row, ti.n0 + ca * 32, ti.group, va, s1, s2, rs, vec_ok, ti.sf_tile + static_cast<int>(rank), quad * 32 + lane);
                 tmem_ld_wait();
@@ -393,7 +397,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 if constexpr (SPLIT)
                     store_partial32(args, ks, row, ti.n0 + cb * 32, row_ok, vb);
                 else if (warp_store && ti.n0 + cb * 32 + 32 <= args.n)
-                    store_chunk32_bf16_warp(args, epi_scratch, row_warp, ti.row_end, ti.n0 + cb * 32, ti.group, vb, s1, s2, rs, lane);
+                    store_warp(row_warp, ti.row_end, ti.n0 + cb * 32, ti.group, vb, rs);
                 else if (row_ok && ti.n0 + cb * 32 < args.n)
                     store_chunk32(args, row, ti.n0 + cb * 32, ti.group, vb, s1, s2, rs, vec_ok, ti.sf_tile + static_cast<int>(rank), quad * 32 + lane);
             }
