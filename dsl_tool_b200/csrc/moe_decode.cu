@@ -1,7 +1,8 @@
-// A whole mixture-of-experts feed-forward layer for a few tokens, in two kernels:
+// A whole mixture-of-experts feed-forward layer for a few tokens, in three kernels:
 //
-//   up     p, e = softmax top-k of the logits;   h[t, s] = silu(g) * u,  (g, u) = pairs of rows of  Wgu[e(t, s)] x[t]
-//   down   y[t, s] = Wdn[e(t, s)] h[t, s];       out[t] = sum over s, in slot order, of p[t, s] * y[t, s]
+//   up       p, e = softmax top-k of the logits;   h[t, s] = silu(g) * u,  (g, u) = pairs of rows of  Wgu[e(t, s)] x[t]
+//   down     y[t, s] = Wdn[e(t, s)] h[t, s]
+//   combine  out[t] = sum over s, in slot order, of p[t, s] * y[t, s]
 //
 // With one or two rows for each chosen expert the layer is the reading of those experts' weights, so everything is arranged round
 // that stream and the activations stay unquantised (nothing would be gained from fewer bits of them).
@@ -14,26 +15,30 @@
 //   * A CTA's steps, tile after tile, are dealt to its 16 warps in equal runs.  A tile that lies inside a run is finished by its
 //     warp; the pieces of the others meet in shared memory after the last step and are added in order.
 //   * The rows of x (or h) that the current expert multiplies are kept in shared memory, as 16-bit values in the order in which the
-//     tensor core's B fragments want them.  Weights go from global memory straight into registers (two steps of four 16-byte
-//     loads a lane in flight while a third is multiplied: 64 KB an SM; three gained nothing), are widened there to f16 or bf16, exactly, and meet the
-//     rows in mma.sync m16n8k16 with fp32 sums.  The order of K inside a step is free as long as both sides agree: lane (g, t) of
-//     a warp holds 16 consecutive bytes of its four rows, every load covers whole 64-byte pieces, and no weight passes through
-//     shared memory.  (tcgen05 would want the widened weight written to shared memory first, for tiles of which at most one column
-//     in eight is used.  The products and the widening are not what bounds: with either left out a layer took as long.)
-//   * Down's results go to scratch by (token, slot); the CTA that delivers a unit's last one adds the slots and writes the output.
-//     Which CTA that is changes nothing: it adds in slot order.
+//     tensor core's B fragments want them.  Weights go from global memory straight into registers (two steps of four 16-byte loads
+//     a lane in flight while a third is multiplied: 64 KB an SM; three, or a ring in shared memory, gained nothing), are widened
+//     there to f16 or bf16, exactly, and meet the rows in mma.sync m16n8k16 with fp32 sums.  The order of K inside a step is free as
+//     long as both sides agree: lane (g, t) of a warp holds 16 consecutive bytes of its four rows, every load covers whole 64-byte
+//     pieces, and no weight passes through shared memory.  (tcgen05 would want the widened weight written to shared memory first,
+//     for tiles of which at most one column in eight is used.  The products and the widening are not what bounds: without either,
+//     8 tokens NVFP4 took 102 us a layer instead of 111.)
+//   * Code that runs once a launch is kept small (loops not unrolled): its instructions come from memory, behind the weights, and
+//     unrolled by the compiler they were two thirds of a kernel (8 tokens NVFP4 102 -> 97 us a layer, FP8 145 -> 141).
+//   * The loads in flight live in the L1, so the kernels ask for as little shared memory as they can do with: with the largest
+//     share of it 8 tokens FP8 took 184 us a layer instead of 142, and kernels that want different shares slow each other
+//     (3 tokens BF16 400 -> 278).
 //
-// Rounding.  Weights are exact in the 16-bit type: E4M3, e2m1 x UE4M3 and int8 in f16, bf16 in bf16; MXFP4's power-of-two scales
-// are taken relative to the largest of a chunk's row and applied to its fp32 sum.  x in bf16 or f16 is exact too: for f16 products
-// a row is scaled by a power of two that brings its largest value just under 2^15, which leaves every value within 2^-39 of that
-// largest one.  An fp32 x and the hidden activation round to 11 bits (f16), or to 16 (two bf16 terms) with bf16 weights - more than
-// the 8 bits of the bf16 hidden activation that the layer of quantised GEMMs passes on.  All sums are fp32.
+// Rounding.  Weights are exact in the 16-bit type: E4M3, e2m1 (x UE4M3) and int8 in f16, bf16 in bf16; FP4 scales that meet the sum
+// of a block instead do so in fp32.  For f16 products a row whose largest magnitude lies in [1, 2^15) is taken as it is: 16-bit
+// values are exact down to 2^-17, off by 2^-25 at most below.  Other rows are scaled by a power of two that brings the largest just
+// under 2^15, which leaves every 16-bit value within 2^-39 of that one.  An fp32 x and the hidden activation round to 11 bits (f16),
+// or to 16 (two bf16 terms) with bf16 weights - more than the 8 bits of the bf16 hidden activation that the layer of quantised GEMMs
+// passes on.  All sums are fp32.
 //
 // Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us (share of the rate at which the chosen experts' bytes can be
-// copied): one token NVFP4 35 (37 %), FP8 40 (57 %); 8 tokens NVFP4 114 (62 %), FP8 128x128 154 (81 %); 16 tokens NVFP4 161 (58 %).
-// 8 experts, top 2, H = 14336, 3 tokens BF16 333 (75 %).  What is left: about 15 us of a layer in which nothing streams (routing and
-// list 3.5 us and the first rows 1.5 us of either kernel, the last sums and counters), and, in FP4, CTAs that wait for the one
-// whose expert has more rows.
+// copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 150 (84 %); 16 tokens NVFP4 129 (73 %).
+// 8 experts, top 2, H = 14336, 3 tokens BF16 294 (85 %).  What is left: about 18 us of a layer in which nothing streams (a kernel's
+// start, routing and list 4 us and the first rows 2 us, of up and of down; the last sums), and CTAs that wait for the slowest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -49,7 +54,8 @@ namespace md {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
-constexpr int SUM_FLOATS = 8 * 36;       // a tile's sums: eight columns of 32 rows, 36 apart (no bank conflicts)
+constexpr int COMBINE_THREADS = 128;
+constexpr int SUM_PITCH = 36;            // a tile's sums: a column of 32 rows for each activation row (36: no bank conflicts)
 constexpr int STEP = 64;                 // bytes of a weight row that a warp takes at once
 constexpr int AHEAD = 3;                 // steps that a lane has registers for: all but one in flight
 constexpr int MIN_STEPS = 4;             // of a tile (short rows: steps without bytes)
@@ -65,9 +71,17 @@ struct Fmt {
     static constexpr int ROWS = FMT == MX ? 4 : 8;       // activation rows that a CTA multiplies at a time, at most
 };
 
+struct Router {
+    const void* logits;          // [tokens, experts]
+    int dtype, tokens, experts, k, renorm;
+    __device__ __forceinline__ float at(size_t i) const {
+        return dtype == DSL_F32 ? static_cast<const float*>(logits)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[i]);
+    }
+};
+
 struct Args {
-    const void* logits;
-    int logits_dtype, tokens, experts, k, renorm;
+    Router route;
+    int tokens, experts, k;
     const void* x;               // up: [tokens, kdim] of x_dtype; down: h, fp32 [entries, kdim]
     int x_dtype;
     const uint8_t* w;            // [experts, n, row_bytes]
@@ -77,15 +91,11 @@ struct Args {
     int units;                   // of 16 rows: 8 for every 128, the last ones possibly without rows
     int entry_cost;              // what starting on an expert costs a CTA, in eighths of a unit against one row
     int steps;                   // of a tile
-    unsigned div_steps, div_grid, div_k;      // 2^32 / steps, / CTAs, / k: see quotient()
+    unsigned div_steps, div_grid, div_k, div_block;      // 2^32 / steps, / CTAs, / k, / block_rows: see quotient()
     int block_rows;              // rows of one expert that a CTA holds at a time
     int parts;                   // 16-bit terms an activation (2 only with bf16 products)
     float* h;                    // up: [entries, n / 2]
     float* y;                    // down: [entries, n]
-    int* arrived;                // down: one counter a unit, zeroed by up
-    int arrived_count;
-    void* out;                   // down: [tokens, n]
-    int out_dtype;
 };
 
 // n / d for n < 2^31, with m = floor((2^32 - 1) / d): the estimate is at most one too small.
@@ -98,7 +108,6 @@ __device__ __forceinline__ int quotient(int n, int d, unsigned m) {
 // Shared-memory tables of the list of work: entry = token * k + slot.
 struct Plan {
     int* ids;          // [entries] expert, or -1
-    float* weights;    // [entries]
     int* order;        // entries sorted by expert, an expert's by token
     int* seg_expert;   // [segments]: an expert with at most block_rows of its rows
     int* seg_first;    //             first place in `order`
@@ -114,48 +123,23 @@ __device__ __forceinline__ uint32_t logit_key(float f) {
     const uint32_t b = __float_as_uint(f + 0.0f);              // one zero
     return f >= -FLT_MAX ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
 }
-__device__ __forceinline__ float key_logit(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-// Softmax over the experts and the k largest, ties to the lower index; the arithmetic of moe_route_kernel (moe.cu), so ids and
-// weights are those of dsl_moe_route.  One warp a token; `v`: room for a row of keys.  An entry without an expert gets -1.
-template <typename T>
-__device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, const Plan& p, int lane) {
-    const T* row = static_cast<const T*>(a.logits) + static_cast<size_t>(t) * a.experts;
+// The k largest logits of token t, ties to the lower index, as in dsl_moe_route: lane j's expert (-1: none left).  One warp; `v`:
+// room for a row of keys.
+__device__ __forceinline__ int choose(const Router& r, int t, uint32_t* v, int lane) {
+    const size_t row = static_cast<size_t>(t) * r.experts;
     uint32_t keep[4];                                          // up to 128 experts stay in registers
-    const bool small = a.experts <= 128;
-    float mx, sum = 0.f;
+    const bool small = r.experts <= 128;
     if (small) {
-        float f[4];
-        uint32_t high = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[i] = lane + 32 * i < a.experts ? static_cast<float>(row[lane + 32 * i]) : -FLT_MAX;
-            keep[i] = lane + 32 * i < a.experts ? logit_key(f[i]) : 0u;
-            high = max(high, keep[i]);
-        }
-        mx = key_logit(__reduce_max_sync(0xFFFFFFFFu, high));  // (nobody's to choose: no entry, whatever the sum)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.experts) sum += expf(f[i] - mx);
+        for (int i = 0; i < 4; ++i) keep[i] = lane + 32 * i < r.experts ? logit_key(r.at(row + lane + 32 * i)) : 0u;
     } else {
-        uint32_t high = 0u;
-        for (int e = lane; e < a.experts; e += 32) {
-            const float f = static_cast<float>(row[e]);
-            v[e] = __float_as_uint(f);
-            high = max(high, logit_key(f));
-        }
-        mx = key_logit(__reduce_max_sync(0xFFFFFFFFu, high));
-        for (int e = lane; e < a.experts; e += 32) {
-            const float f = __uint_as_float(v[e]);
-            sum += expf(f - mx);
-            v[e] = logit_key(f);
-        }
+#pragma unroll 1
+        for (int e = lane; e < r.experts; e += 32) v[e] = logit_key(r.at(row + e));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    uint32_t my_key = 0u;                                      // lane j keeps the j-th choice
-    int my_e = -1;
-    for (int j = 0; j < a.k; ++j) {
+    int mine = -1;
+#pragma unroll 1
+    for (int j = 0; j < r.k; ++j) {
         uint32_t best = 0u;
         unsigned bi = 0x7FFFFFFFu;
         if (small) {
@@ -163,7 +147,8 @@ __device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, c
             for (int i = 0; i < 4; ++i)
                 if (keep[i] > best) { best = keep[i]; bi = lane + 32 * i; }
         } else {
-            for (int e = lane; e < a.experts; e += 32) {
+#pragma unroll 1
+            for (int e = lane; e < r.experts; e += 32) {
                 const uint32_t key = v[e];
                 if (key > best) { best = key; bi = e; }
             }
@@ -171,7 +156,7 @@ __device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, c
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
         if (top == 0u) break;                                  // uniform: nobody has one left
         const int e = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, best == top ? bi : 0x7FFFFFFFu));
-        if (lane == j) { my_key = top; my_e = e; }
+        if (lane == j) mine = e;
         if (small) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -180,21 +165,34 @@ __device__ __forceinline__ void route_token(const Args& a, int t, uint32_t* v, c
             v[e] = 0u;                                         // its own lane's alone to read
         }
     }
-    const float pr = my_e >= 0 ? __fdiv_rn(expf(key_logit(my_key) - mx), sum) : 0.f;
+    return mine;
+}
+
+// Weight of lane j's choice `e`: softmax over all experts, with the arithmetic of moe_route_kernel (moe.cu), so that it is
+// dsl_moe_route's.  One warp.
+__device__ __forceinline__ float weigh(const Router& r, int t, int e, int lane) {
+    const size_t row = static_cast<size_t>(t) * r.experts;
+    const float own = e >= 0 ? r.at(row + e) + 0.0f : 0.f, mx = __shfl_sync(0xFFFFFFFFu, own, 0);      // the first is the largest
+    float sum = 0.f;
+#pragma unroll 1
+    for (int i = lane; i < r.experts; i += 32) sum += expf(r.at(row + i) - mx);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const float pr = e >= 0 ? __fdiv_rn(expf(own - mx), sum) : 0.f;
+    if (!r.renorm) return pr;
     float psum = 0.f;
-    for (int j = 0; j < a.k; ++j) psum += __shfl_sync(0xFFFFFFFFu, pr, j);
-    if (lane < a.k) {
-        p.ids[t * a.k + lane] = my_e;
-        p.weights[t * a.k + lane] = a.renorm ? __fdiv_rn(pr, psum) : pr;
-        if (my_e >= 0) atomicOr(&p.tokens[my_e], 1u << t);
-    }
+#pragma unroll 1
+    for (int j = 0; j < r.k; ++j) psum += __shfl_sync(0xFFFFFFFFu, pr, j);
+    return __fdiv_rn(pr, psum);
 }
 
 // Cost of a unit, in eighths, against so many rows.  Measured a unit, us: NVFP4 1 / 2 / 3 rows 0.89 / 1.06 / 1.06 (K = 4096), MXFP4
 // 1 / 2 / 3 / 4 rows 0.67 / 0.67 / 0.87 / 0.86 (K = 2912), FP8 128x128 1.31 whatever the rows.  In the shares: 8 tokens NVFP4 142 ->
 // 123 us a layer, 16 tokens MXFP4 196 -> 172.
 template <int FMT>
-__device__ __forceinline__ int unit_cost(int rows) { return FMT == NV ? (rows == 1 ? 8 : 9) : (FMT == MX && rows > 2 ? 10 : 8); }
+__device__ __forceinline__ bool heavy(int rows) { return FMT == NV ? rows > 1 : FMT == MX && rows > 2; }
+template <int FMT>
+__device__ __forceinline__ int unit_cost(int rows) { return heavy<FMT>(rows) ? (FMT == NV ? 9 : 10) : 8; }
 // Units that `cost` pays for.
 template <int FMT>
 __device__ __forceinline__ int units_for(int cost, int rows) {
@@ -207,51 +205,57 @@ __device__ __forceinline__ int units_for(int cost, int rows) {
 template <int FMT>
 __device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work, int* s_misc, int& begin, int& end, int& seg) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
     for (int e = threadIdx.x; e < a.experts; e += THREADS) p.tokens[e] = 0u;
     __syncthreads();
+#pragma unroll 1
     for (int t = warp; t < a.tokens; t += WARPS) {
-        if (a.logits_dtype == DSL_F32) route_token<float>(a, t, work + warp * a.experts, p, lane);
-        else route_token<__nv_bfloat16>(a, t, work + warp * a.experts, p, lane);
+        const int e = choose(a.route, t, work + warp * a.experts, lane);
+        if (lane < a.k) {
+            p.ids[t * a.k + lane] = e;
+            if (e >= 0) atomicOr(&p.tokens[e], 1u << t);
+        }
     }
     __syncthreads();
     if (warp == 0) {
-        // experts 32 at a time: their places and segments
-        int rows = 0, segments = 0, start = 0;
-        for (int e0 = 0; e0 < a.experts; e0 += 32) {
-            const int e = e0 + lane;
-            const int c = e < a.experts ? __popc(p.tokens[e]) : 0;
-            const int b = (c + a.block_rows - 1) / a.block_rows;
-            int run = c | (b << 16);                           // both sums at once: at most 1024 each
-            const int full = a.entry_cost + a.units * unit_cost<FMT>(a.block_rows), rest = c - (b - 1) * a.block_rows;
-            const int cost = b > 0 ? (b - 1) * full + a.entry_cost + a.units * unit_cost<FMT>(rest) : 0;
-            int run_cost = cost;
+        // experts 32 at a time: their places and segments.  Three sums in a word: rows (at most 1024), segments (1024), segments
+        // that cost more (two rows at least, so 512).
+        const int plain = a.entry_cost + a.units * 8, extra = a.units * (FMT == NV ? 1 : 2), full_heavy = heavy<FMT>(a.block_rows) ? 1 : 0;
+        uint32_t before = 0u;
+#pragma unroll 1
+        for (int e = lane; e - lane < a.experts; e += 32) {
+            const int c = e < a.experts ? __popc(p.tokens[e]) : 0, b = quotient(c + a.block_rows - 1, a.block_rows, a.div_block);
+            const int more = b > 0 ? (b - 1) * full_heavy + (heavy<FMT>(c - (b - 1) * a.block_rows) ? 1 : 0) : 0;
+            const uint32_t what = static_cast<uint32_t>(c | (b << 11) | (more << 22));
+            uint32_t run = before + what;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xFFFFFFFFu, run, o), vc = __shfl_up_sync(0xFFFFFFFFu, run_cost, o);
-                if (lane >= o) {
-                    run += v;
-                    run_cost += vc;
-                }
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, run, o);
+                if (lane >= o) run += v - before;
             }
-            const int first = rows + (run & 0xFFFF) - c, s0 = segments + (run >> 16) - b;
+            const uint32_t at = run - what;
+            int first = at & 0x7FF, place = at >> 11 & 0x7FF, start = place * plain + static_cast<int>(at >> 22) * extra;
             if (c > 0) p.base[e] = first;
-            for (int i = 0; i < b; ++i) {
-                p.seg_expert[s0 + i] = e;
-                p.seg_first[s0 + i] = first + i * a.block_rows;
-                p.seg_rows[s0 + i] = min(a.block_rows, c - i * a.block_rows);
-                p.seg_start[s0 + i] = start + run_cost - cost + i * full;
+#pragma unroll 1
+            for (int left = c; left > 0; left -= a.block_rows) {
+                p.seg_expert[place] = e;
+                p.seg_first[place] = first;
+                p.seg_rows[place] = min(a.block_rows, left);
+                p.seg_start[place] = start;
+                first += a.block_rows;
+                ++place;
+                start += plain + full_heavy * extra;
             }
-            run = __shfl_sync(0xFFFFFFFFu, run, 31);
-            rows += run & 0xFFFF;
-            segments += run >> 16;
-            start += __shfl_sync(0xFFFFFFFFu, run_cost, 31);
+            before = __shfl_sync(0xFFFFFFFFu, run, 31);
         }
+        const int segments = before >> 11 & 0x7FF, start = segments * plain + static_cast<int>(before >> 22) * extra;
         if (lane == 0) {
             s_misc[0] = segments;
             p.seg_start[segments] = start;
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int t = warp; t < a.tokens; t += WARPS) {
         const int e = lane < a.k ? p.ids[t * a.k + lane] : -1;
         if (e >= 0) p.order[p.base[e] + __popc(p.tokens[e] & ((1u << t) - 1u))] = t * a.k + lane;
@@ -261,10 +265,11 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p, uint32_t* work
     const int share = quotient(places, ctas, a.div_grid), more_than = places - share * ctas;
     begin = bid * share + min(bid, more_than);
     end = begin + share + (bid < more_than ? 1 : 0);
+#pragma unroll 1
     for (int i = threadIdx.x; i < p.segments; i += THREADS)
-        if (p.seg_start[i] <= begin && begin < p.seg_start[i + 1]) s_misc[2] = i;
+        if (p.seg_start[i] <= begin && begin < p.seg_start[i + 1]) s_misc[1] = i;
     __syncthreads();
-    seg = s_misc[2];
+    seg = s_misc[1];
 }
 
 // ---- 16-bit products ---------------------------------------------------------------------------------------------------------------
@@ -287,6 +292,12 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w) {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
     return r;
 }
+// two UE8M0 bytes (low 16 bits of w) -> two bf16: 2^(byte - 127), a subnormal for 0, and NaN for 255
+__device__ __forceinline__ uint32_t widen_ue8m0(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
 // byte I of w: two e2m1 nibbles -> two f16 (low nibble in the low half)
 template <int I>
 __device__ __forceinline__ uint32_t widen_e2m1(uint32_t w) {
@@ -304,13 +315,11 @@ __device__ __forceinline__ uint32_t widen_int8(uint32_t biased, uint32_t selecto
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// 16 bytes that are read once.  Where streaming bounds (all but the FP4 formats) the L2 is asked for 256 bytes of the row, which the
-// warp comes to in its next steps: the memory reads longer pieces (8 tokens FP8 171 -> 157 us a layer, 3 tokens BF16 390 -> 331).
-template <int FMT>
+// 16 bytes that are read once.  The L2 is asked for 256 bytes of the row, which the warp comes to in its next steps: the memory reads
+// longer pieces (8 tokens FP8 171 -> 157 us a layer, NVFP4 111 -> 107, 3 tokens BF16 390 -> 331).
 __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
     uint4 r;
-    if (Fmt<FMT>::FP4) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    else asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
 // Scale bytes: past the L1 too, which the lines of a whole atom would run through (8 tokens NVFP4 124 -> 114 us a layer).
@@ -329,24 +338,25 @@ struct Piece {
     uint4 s;                             // NV, MX: word j = the scale bytes of row j's atom
     float group;                         // F8G: scale of the step's 128-element group
 
-    // `row`: row j = 0 of this lane, `pitch`: 32 rows on; `rows`: bit j = row j exists and is this CTA's
-    __device__ __forceinline__ void load(const Args& a, const uint8_t* row, int pitch, unsigned rows, const uint8_t* scale, int step, int t) {
-        const int at = step * STEP + t * 16;
-        const bool in = at < a.row_bytes;
+    // `row`: row j = 0 of this lane, `rows`: from there to its rows.  Behind a row's end its last piece comes again, against zeros:
+    // a NaN that it holds is in the row's sum already (bf16, whose infinities would make one, gets zeros).
+    __device__ __forceinline__ void load(const Args& a, const uint8_t* row, const unsigned (&rows)[4], const uint8_t* scale, int step, int t) {
+        const int there = step * STEP + t * 16, at = min(there, a.row_bytes - 16);
+        const uint8_t* p = row + at;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (in && (rows >> j & 1u)) w[j] = load_stream<FMT>(row + static_cast<size_t>(static_cast<unsigned>(j * pitch)) + at);
+            w[j] = load_stream(p + rows[j]);
+            if (FMT == BF && there != at) w[j] = make_uint4(0u, 0u, 0u, 0u);
         }
-        // NV: two blocks a piece, so atom piece / 2; MX: one, atom piece / 4, which all lanes of a quad need for its maximum
-        if (FMT == NV) s = in ? load_table(scale + static_cast<size_t>(at >> 5) * 512) : make_uint4(0u, 0u, 0u, 0u);
-        if (FMT == MX) s = step * STEP < a.row_bytes ? load_table(scale + static_cast<size_t>(step) * 512) : make_uint4(0u, 0u, 0u, 0u);
+        // NV: two blocks a piece, so atom piece / 2; MX: one, atom piece / 4 (the step)
+        if (FMT == NV) s = load_table(scale + static_cast<size_t>(at >> 5) * 512);
+        if (FMT == MX) s = load_table(scale + static_cast<size_t>(min(step, (a.row_bytes - 1) / STEP)) * 512);
         if (FMT == F8G) group = step * STEP < a.row_bytes ? __ldg(reinterpret_cast<const float*>(scale) + (step >> 1)) : 0.f;
     }
 };
 
-// A fragment of two k16 steps from vector v of a lane's pieces of two rows (16 consecutive values of eight lanes' rows ...): the
-// widened weights as they are, without FP4 scales.
+// A fragments of two k16 steps (a0, a1) from vector v, eight values each, of a lane's pieces of two rows: the widened weights
+// without FP4 scales.
 template <int FMT>
 __device__ __forceinline__ void widen_rows(const uint4& q0, const uint4& q1, int v, uint32_t (&a0)[4], uint32_t (&a1)[4]) {
 #pragma unroll
@@ -468,11 +478,9 @@ __device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* 
             s0 = f.x;
             s1 = f.y;
         } else {
-            // 2^(byte - 127): the byte as an exponent, subnormal for 0, and 255 (infinity so far) is NaN
-            s0 = __uint_as_float(max((two & 255u) << 23, 0x00400000u));
-            s1 = __uint_as_float(max((two >> 8 & 255u) << 23, 0x00400000u));
-            s0 = fmaf(0.0f, s0, s0);
-            s1 = fmaf(0.0f, s1, s1);
+            const uint32_t h = widen_ue8m0(two);
+            s0 = __uint_as_float(h << 16);
+            s1 = __uint_as_float(h & 0xFFFF0000u);
         }
 #pragma unroll
         for (int k = 0; k < SETS; ++k) {
@@ -529,8 +537,10 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
     const int dtype = DOWN ? DSL_F32 : a.x_dtype;
     if (threadIdx.x < rows) s_amax[threadIdx.x] = 0u;
     __syncthreads();
+#pragma unroll 1
     for (bool again = false;; again = true) {
         bool more = false;
+#pragma unroll 1
         for (int r = 0; r < rows; ++r) {
             const int entry = p.order[first + r];
             const size_t src = static_cast<size_t>(DOWN ? entry : quotient(entry, a.k, a.div_k)) * a.kdim;
@@ -541,7 +551,7 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
             }
             if (threadIdx.x == 0) s_inverse[r] = inverse;
             uint32_t m = 0u;
-#pragma unroll 4
+#pragma unroll 1
             for (int v = threadIdx.x; v < vectors; v += THREADS) {
                 float f[8];
                 if (v * 8 < a.kdim) {
@@ -577,10 +587,12 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
             }
         }
         if (F::FP4 && !again)
+#pragma unroll 1
             for (int v = threadIdx.x; v < part_bytes / 16; v += THREADS)
                 *reinterpret_cast<uint4*>(dst + static_cast<size_t>(rows) * pitch + v * 16) = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
         if (!scaled || again) return;
+#pragma unroll 1
         for (int r = 0; r < rows; ++r) more |= !fits_f16(s_amax[r]);
         if (!more) return;
     }
@@ -588,17 +600,16 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
 
 // ---- shared memory ----------------------------------------------------------------------------------------------------------------
 struct Layout {
-    int ids, weights, order, seg_expert, seg_first, seg_rows, seg_start, chosen, base, misc, sums, rows, total;
+    int ids, order, seg_expert, seg_first, seg_rows, seg_start, chosen, base, misc, sums, rows, total;
     int pitch, part_bytes;
 };
-// `elems`: elements of a weight in 16 bytes; the rows' region doubles as the router's room and the list of finished units.
+// `elems`: elements of a weight in 16 bytes; the rows' region doubles as the router's room.
 __host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) {
     Layout l;
     const int entries = a.tokens * a.k;
     int at = 0;
     auto take = [&](int bytes) { const int here = at; at += (bytes + 15) / 16 * 16; return here; };
     l.ids = take(entries * 4);
-    l.weights = take(entries * 4);
     l.order = take(entries * 4);
     l.seg_expert = take(entries * 4);
     l.seg_first = take(entries * 4);
@@ -606,14 +617,13 @@ __host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) 
     l.seg_start = take((entries + 1) * 4);
     l.chosen = take(a.experts * 4);
     l.base = take(a.experts * 4);
-    l.misc = take(16 + 2 * 8 * 4);                                     // three counters; amax of the rows, their inverse factors
-    l.sums = take(3 * WARPS * SUM_FLOATS * 4);                         // a run's first piece of a tile, its last one, a whole one
+    l.misc = take(16 + 2 * 8 * 4);                                     // two numbers; amax of the rows, their inverse factors
+    l.sums = take(3 * WARPS * a.block_rows * SUM_PITCH * 4);           // a run's first piece of a tile, its last one, a whole one
     l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 128
     l.pitch = l.part_bytes * a.parts + 64;                             // two rows start half a bank round apart
     l.rows = take(0);
     int room = (a.block_rows + (fp4 ? 1 : 0)) * l.pitch;
     if (room < WARPS * a.experts * 4) room = WARPS * a.experts * 4;
-    if (room < a.units * 4) room = a.units * 4;
     l.total = l.rows + room;
     return l;
 }
@@ -634,7 +644,6 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     const md::Layout l = md::layout_of(a, F::ELEMS, F::FP4);
     md::Plan plan;
     plan.ids = reinterpret_cast<int*>(smem + l.ids);
-    plan.weights = reinterpret_cast<float*>(smem + l.weights);
     plan.order = reinterpret_cast<int*>(smem + l.order);
     plan.seg_expert = reinterpret_cast<int*>(smem + l.seg_expert);
     plan.seg_first = reinterpret_cast<int*>(smem + l.seg_first);
@@ -642,7 +651,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     plan.seg_start = reinterpret_cast<int*>(smem + l.seg_start);
     plan.tokens = reinterpret_cast<uint32_t*>(smem + l.chosen);
     plan.base = reinterpret_cast<int*>(smem + l.base);
-    int* s_misc = reinterpret_cast<int*>(smem + l.misc);               // [0] segments, [1] units that this CTA completes, [2] its first segment
+    int* s_misc = reinterpret_cast<int*>(smem + l.misc);               // [0] segments, [1] this CTA's first one
     uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + l.misc + 16);
     float* s_inverse = reinterpret_cast<float*>(smem + l.misc + 16 + 32);
     float* s_sums = reinterpret_cast<float*>(smem + l.sums);
@@ -654,8 +663,6 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         // Launched as a dependent, and lets its own successor be placed once everything before it is complete.
         griddep_wait();
         griddep_launch_dependents();
-        if (blockIdx.x == 0)
-            for (int i = threadIdx.x; i < a.arrived_count; i += THREADS) a.arrived[i] = 0;
     }
     // f16 rows are what they are, bf16 ones as bf16 too; the second bf16 term of an fp32 value wants room below the first
     const bool scaled = DOWN || a.x_dtype == DSL_F32 || (a.x_dtype == DSL_BF16 && !F::BF16);
@@ -664,7 +671,6 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     // the next, and has to fetch that one's rows, is dealt less.
     int begin, end, seg0;
     md::make_plan<FMT>(a, plan, reinterpret_cast<uint32_t*>(s_rows), s_misc, begin, end, seg0);
-    const int ctas = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
     bool waited = !DOWN;
     auto units_of = [&](int seg, int& unit0, int& unit1) {
         const int start = plan.seg_start[seg], rows = plan.seg_rows[seg];
@@ -672,6 +678,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         unit1 = md::units_for<FMT>(min(end, plan.seg_start[seg + 1]) - start - a.entry_cost, rows);
     };
 
+#pragma unroll 1
     for (int seg = seg0; begin < end && seg < plan.segments && plan.seg_start[seg] < end; ++seg) {
         int unit0, unit1;
         units_of(seg, unit0, unit1);
@@ -685,15 +692,15 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
 
         // Where the loads are: up to AHEAD - 1 steps before the products.
         static_assert(md::AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
-        const int pitch = 32 * a.row_bytes;
         int l_at = run0, l_step = step, l_tile = tile0 + tile;
         const uint8_t *l_row = nullptr, *l_scale = nullptr;
-        unsigned l_rows = 0;
+        unsigned l_rows[4] = {0u, 0u, 0u, 0u};      // from l_row to the lane's rows: where one is not there or not this CTA's, to another
         auto locate = [&]() {
-            const int r0 = md::row_of(l_tile, g, 0);
+            const int r0 = min(md::row_of(l_tile, g, 0), a.n - 1), last = (a.n - 1 - r0) / 32;
             l_row = a.w + (static_cast<size_t>(expert) * a.n + r0) * a.row_bytes;
-            const unsigned in = r0 >= a.n ? 0u : min(4u, static_cast<unsigned>(a.n - r0 + 31) / 32u);      // rows that the weight has
-            l_rows = ((1u << in) - 1u) & (2 * l_tile < unit0 ? 0xCu : 0xFu) & (2 * l_tile + 1 >= unit1 ? 0x3u : 0xFu);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                l_rows[j] = static_cast<unsigned>(min(last, min(max(j, 2 * l_tile < unit0 ? 2 : 0), 2 * l_tile + 1 >= unit1 ? 1 : 3))) * 32u * a.row_bytes;
             const size_t block = static_cast<size_t>(expert) * ((a.n + 127) / 128) + (l_tile >> 2);
             if (FMT == md::NV || FMT == md::MX) l_scale = a.scale + block * a.katoms * 512 + ((l_tile & 3) * 8 + g) * 16;
             if (FMT == md::F8G) l_scale = a.scale + block * (a.kdim / 128) * 4;
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         md::Piece<FMT> buf[md::AHEAD];
         auto fetch = [&](md::Piece<FMT>& p) {
             if (l_at < run1) {
-                p.load(a, l_row, pitch, l_rows, l_scale, l_step, t4);
+                p.load(a, l_row, l_rows, l_scale, l_step, t4);
                 ++l_at;
                 if (++l_step == a.steps) {
                     l_step = 0;
@@ -728,7 +735,8 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         clear();
         // The sums of a tile that ends, or of the piece of it that the run has, go to one of the warp's three places in shared
         // memory: 0 a tile that begins before the run, 1 one that ends behind it, 2 a whole one, which is finished at once.
-        float* mine = s_sums + warp * (3 * md::SUM_FLOATS);
+        const int sum_floats = a.block_rows * md::SUM_PITCH;
+        float* mine = s_sums + warp * (3 * sum_floats);
         // Everything from here to the segment's end, for one way of forming the products (sets: 0 rows as columns, else blocks).
         auto stream = [&](auto way) {
             constexpr int SETS = decltype(way)::value;
@@ -756,12 +764,12 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 const int from = tl * a.steps, to = from + a.steps;
                 const int place = from < run0 ? 0 : (to > run1 ? 1 : 2);
                 if (place == 2) whole = tl;
-                float* d = mine + place * md::SUM_FLOATS + g;
+                float* d = mine + place * sum_floats + g;
                 if constexpr (SETS == 0) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        d[(2 * t4) * 36 + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2];
-                        d[(2 * t4 + 1) * 36 + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2 + 1];
+                        if (2 * t4 < rows) d[(2 * t4) * md::SUM_PITCH + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2];
+                        if (2 * t4 + 1 < rows) d[(2 * t4 + 1) * md::SUM_PITCH + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2 + 1];
                     }
                 } else {
 #pragma unroll
@@ -774,16 +782,19 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                             if (FMT == md::NV) v[j] += __shfl_xor_sync(0xFFFFFFFFu, v[j], 2);
                         }
                         if (FMT == md::NV) {             // lane t has row j = t to write, of column k
-                            d[k * 36 + 8 * t4] = t4 == 0 ? v[0] : (t4 == 1 ? v[1] : (t4 == 2 ? v[2] : v[3]));
+                            d[k * md::SUM_PITCH + 8 * t4] = t4 == 0 ? v[0] : (t4 == 1 ? v[1] : (t4 == 2 ? v[2] : v[3]));
                         } else {                         // rows t % 2 * 2 and + 1, of column 2 k + t / 2
-                            float* e = d + (2 * k + (t4 >> 1)) * 36 + 16 * (t4 & 1);
-                            e[0] = t4 & 1 ? v[2] : v[0];
-                            e[8] = t4 & 1 ? v[3] : v[1];
+                            float* e = d + (2 * k + (t4 >> 1)) * md::SUM_PITCH + 16 * (t4 & 1);
+                            if (2 * k + (t4 >> 1) < rows) {
+                                e[0] = t4 & 1 ? v[2] : v[0];
+                                e[8] = t4 & 1 ? v[3] : v[1];
+                            }
                         }
                     }
                 }
                 clear();
             };
+#pragma unroll 1
             for (bool met = false;;) {
                 int place = 2, others = warp + 1;          // whose pieces make up the tile that is finished below
                 if (at < run1) {
@@ -825,10 +836,12 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 if (FMT == md::F8) common = *reinterpret_cast<const float*>(a.scale);
                 if (FMT == md::NV) common = *a.global_scale;
                 if (FMT == md::I8) common = ours ? __ldg(reinterpret_cast<const float*>(a.scale) + static_cast<size_t>(expert) * a.n + r) : 0.f;
+#pragma unroll 1
                 for (int c = 0; c < rows; ++c) {
-                    float v = mine[place * md::SUM_FLOATS + c * 36 + lane];
+                    float v = mine[place * sum_floats + c * md::SUM_PITCH + lane];
+#pragma unroll 1
                     for (int w = warp + 1; w < others; ++w)
-                        if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * md::SUM_FLOATS) + c * 36 + lane];      // (not of an empty run)
+                        if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * sum_floats) + c * md::SUM_PITCH + lane];      // (not of an empty run)
                     v = v * s_inverse[c] * common;
                     const int entry = plan.order[first + c];
                     if (DOWN) {
@@ -854,70 +867,66 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         }
     }
 
-    if (DOWN) {
-        if (!waited) {           // a CTA without work: the counters and the output are still up's
-            griddep_wait();
-            griddep_launch_dependents();
-        }
-        // Every result of this CTA is in memory before it counts itself in.
-        __threadfence();
-        if (threadIdx.x == 0) s_misc[1] = 0;
-        __syncthreads();
-        int* s_list = reinterpret_cast<int*>(s_rows);               // the units that this CTA completes
-        for (int seg = seg0; begin < end && seg < plan.segments && plan.seg_start[seg] < end; ++seg) {
-            int unit0, unit1;
-            units_of(seg, unit0, unit1);
-            for (int unit = unit0 + threadIdx.x; unit < unit1; unit += THREADS)
-                if (atomicAdd(&a.arrived[unit], 1) == plan.segments - 1) s_list[atomicAdd(&s_misc[1], 1)] = unit;
-        }
-        __syncthreads();
-        __threadfence();
-        // With no entry at all (every logit masked) nobody counts: the CTAs share the zeros.  Four columns a thread: half of a
-        // row group of eight.
-        const bool none = plan.segments == 0, vec = a.n % 4 == 0;
-        const int listed = none ? (a.units - bid + ctas - 1) / ctas : s_misc[1];
-        const int each = a.tokens * 4;
-        for (int i = threadIdx.x; i < listed * each; i += THREADS) {
-            const int which = i / each, in = i - which * each, t = in >> 2;
-            const int unit = none ? bid + which * ctas : s_list[which];
-            const int col = md::row_of(unit >> 1, (in & 1) * 4, (unit & 1) * 2 + (in >> 1 & 1));
-            if (col >= a.n) continue;
-            const float* y = a.y + static_cast<size_t>(t) * a.k * a.n + col;
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int j0 = 0; j0 < a.k; j0 += 8) {         // eight slots' loads in flight
-                float4 u[8];
-                float p[8];
+    if (DOWN && !waited) {       // a CTA without work: the last kernel relies on up's being complete
+        griddep_wait();
+        griddep_launch_dependents();
+    }
+}
+
+// out[t] = sum over s of p[t, s] * y[t, s], in slot order, in fp32.  A CTA has 512 columns of a token, a thread four of them, eight
+// slots' loads in flight.  Choices and weights it makes for itself while down still runs.  A kernel of its own, since a unit is
+// complete only when its last expert is: added by the CTA that delivers a unit's last result (counters), the sums fell to the CTAs
+// that finished last, 16 tokens MXFP4 up to 115 units, 25 us.
+__global__ void __launch_bounds__(md::COMBINE_THREADS) moe_decode_combine_kernel(const md::Router r, const float* __restrict__ y, int n,
+                                                                                 void* out, int out_dtype) {
+    __shared__ uint32_t s_keys[DSL_MAX_GROUPS];
+    __shared__ int s_ids[32];
+    __shared__ float s_weights[32];
+    const int t = blockIdx.y, k = r.k, col = (blockIdx.x * md::COMBINE_THREADS + threadIdx.x) * 4;
+    if (threadIdx.x < 32) {
+        const int e = md::choose(r, t, s_keys, threadIdx.x);
+        s_ids[threadIdx.x] = e;                      // slots past k: none
+        s_weights[threadIdx.x] = md::weigh(r, t, e, threadIdx.x);
+    }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch_dependents();
+    if (col >= n) return;
+    const bool vec = n % 4 == 0;
+    const float* row = y + static_cast<size_t>(t) * k * n + col;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int j0 = 0; j0 < k; j0 += 8) {
+        float4 u[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool in = j0 + j < a.k && plan.ids[t * a.k + j0 + j] >= 0;
-                    const float* q = y + static_cast<size_t>(j0 + j) * a.n;
-                    p[j] = in ? plan.weights[t * a.k + j0 + j] : 0.f;
-                    u[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (in && vec) {
-                        u[j] = __ldcg(reinterpret_cast<const float4*>(q));
-                    } else if (in) {
-                        u[j].x = __ldcg(q);
-                        if (col + 1 < a.n) u[j].y = __ldcg(q + 1);
-                        if (col + 2 < a.n) u[j].z = __ldcg(q + 2);
-                        if (col + 3 < a.n) u[j].w = __ldcg(q + 3);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    s[0] = fmaf(p[j], u[j].x, s[0]);
-                    s[1] = fmaf(p[j], u[j].y, s[1]);
-                    s[2] = fmaf(p[j], u[j].z, s[2]);
-                    s[3] = fmaf(p[j], u[j].w, s[3]);
-                }
-            }
-            const size_t to = static_cast<size_t>(t) * a.n + col;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (col + c >= a.n) break;
-                if (a.out_dtype == DSL_BF16) static_cast<__nv_bfloat16*>(a.out)[to + c] = __float2bfloat16_rn(s[c]);
-                else static_cast<float*>(a.out)[to + c] = s[c];
+        for (int j = 0; j < 8; ++j) {
+            const int slot = min(j0 + j, k - 1);
+            const float* q = row + static_cast<size_t>(slot) * n;
+            if (vec) {
+                u[j] = __ldcg(reinterpret_cast<const float4*>(q));
+            } else {
+                u[j] = make_float4(__ldcg(q), 0.f, 0.f, 0.f);
+                if (col + 1 < n) u[j].y = __ldcg(q + 1);
+                if (col + 2 < n) u[j].z = __ldcg(q + 2);
+                if (col + 3 < n) u[j].w = __ldcg(q + 3);
             }
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (s_ids[j0 + j] < 0) continue;         // not written
+            const float p = s_weights[j0 + j];
+            s[0] = fmaf(p, u[j].x, s[0]);
+            s[1] = fmaf(p, u[j].y, s[1]);
+            s[2] = fmaf(p, u[j].z, s[2]);
+            s[3] = fmaf(p, u[j].w, s[3]);
+        }
+    }
+    const size_t to = static_cast<size_t>(t) * n + col;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (col + c >= n) break;
+        if (out_dtype == DSL_BF16) static_cast<__nv_bfloat16*>(out)[to + c] = __float2bfloat16_rn(s[c]);
+        else static_cast<float*>(out)[to + c] = s[c];
     }
 }
 
@@ -950,7 +959,14 @@ static bool plan_launch(Args& a, int format, int* smem_bytes) {
         fits = r;
     }
     a.block_rows = fits;
+    if (fits > 0) a.div_block = inverse(fits);
     return fits > 0;
+}
+
+// As little shared memory as a launch needs.
+template <typename K>
+static cudaError_t prefer_l1(K kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxL1);
 }
 
 template <int FMT, bool DOWN>
@@ -961,6 +977,8 @@ static int launch_one(Args& a, int smem_bytes, int sms, cudaStream_t st) {
     if (attr_set.v[dev].load(std::memory_order_acquire) == 0) {
         const cudaError_t e = cudaFuncSetAttribute(moe_decode_kernel<FMT, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
         if (e != cudaSuccess) return static_cast<int>(e);
+        const cudaError_t c = prefer_l1(moe_decode_kernel<FMT, DOWN>);
+        if (c != cudaSuccess) return static_cast<int>(c);
         attr_set.v[dev].store(1, std::memory_order_release);
     }
     a.div_grid = 0xFFFFFFFFu / static_cast<unsigned>(sms);
@@ -1000,9 +1018,29 @@ static int launch_fmt(int format, Args& up, Args& down, int sms, cudaStream_t st
     int bytes_up = 0, bytes_down = 0;
     if (!plan_launch(up, format, &bytes_up) || !plan_launch(down, format, &bytes_down))
         return DSL_ERR_TOO_LARGE;
-    up.arrived_count = down.units;
     const int rc = launch_one<FMT, false>(up, bytes_up, sms, st);
     return rc != 0 ? rc : launch_one<FMT, true>(down, bytes_down, sms, st);
+}
+
+static int launch_combine(const Router& r, const float* y, int n, void* out, int out_dtype, cudaStream_t st) {
+    static PerDeviceInt attr_set;
+    const int dev = current_device_slot();
+    if (dev < 0) return static_cast<int>(cudaErrorInvalidDevice);
+    if (attr_set.v[dev].load(std::memory_order_acquire) == 0) {
+        const cudaError_t e = prefer_l1(moe_decode_combine_kernel);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        attr_set.v[dev].store(1, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(((n + 3) / 4 + COMBINE_THREADS - 1) / COMBINE_THREADS), static_cast<unsigned>(r.tokens));
+    cfg.blockDim = dim3(COMBINE_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, moe_decode_combine_kernel, r, y, n, out, out_dtype));
 }
 
 // What the entry point takes; 0 or DSL_ERR_*.
@@ -1040,7 +1078,7 @@ using namespace dsl;
 extern "C" size_t dsl_moe_decode_scratch_bytes(const dsl_weight* gate_up, const dsl_weight* down, int tokens, int k, int x_dtype) {
     if (md::check(gate_up, down, tokens, k, x_dtype) != 0 || tokens == 0) return 0;
     const size_t entries = static_cast<size_t>(tokens) * k;
-    return md::up256(entries * down->k * 4) + md::up256(entries * down->n * 4) + md::up256((down->n + 127) / 128 * 8 * 4ull);
+    return md::up256(entries * down->k * 4) + md::up256(entries * down->n * 4);
 }
 
 extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, int logits_dtype, int tokens, int k, int renorm,
@@ -1065,27 +1103,22 @@ extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, in
     uint8_t* base = static_cast<uint8_t*>(scratch);
     float* h = reinterpret_cast<float*>(base);
     float* y = reinterpret_cast<float*>(base + md::up256(entries * down->k * 4));
-    int* arrived = reinterpret_cast<int*>(base + md::up256(entries * down->k * 4) + md::up256(entries * down->n * 4));
-    for (md::Args* a : {&up, &dn}) {
-        a->logits = logits;
-        a->logits_dtype = logits_dtype;
-        a->renorm = renorm;
-        a->arrived = arrived;
-    }
+    const md::Router route = {logits, logits_dtype, tokens, gate_up->groups, k, renorm};
+    up.route = route;
+    dn.route = route;
     up.x = x;
     up.h = h;
     dn.x = h;
     dn.y = y;
-    dn.out = out;
-    dn.out_dtype = out_dtype;
     const int sms = sm_count();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (format) {
-        case DSL_W_FP8: return md::launch_fmt<md::F8>(format, up, dn, sms, st);
-        case DSL_W_FP8_BLOCK128: return md::launch_fmt<md::F8G>(format, up, dn, sms, st);
-        case DSL_W_INT8: return md::launch_fmt<md::I8>(format, up, dn, sms, st);
-        case DSL_W_NVFP4: return md::launch_fmt<md::NV>(format, up, dn, sms, st);
-        case DSL_W_MXFP4: return md::launch_fmt<md::MX>(format, up, dn, sms, st);
-        default: return md::launch_fmt<md::BF>(format, up, dn, sms, st);
+        case DSL_W_FP8: rc = md::launch_fmt<md::F8>(format, up, dn, sms, st); break;
+        case DSL_W_FP8_BLOCK128: rc = md::launch_fmt<md::F8G>(format, up, dn, sms, st); break;
+        case DSL_W_INT8: rc = md::launch_fmt<md::I8>(format, up, dn, sms, st); break;
+        case DSL_W_NVFP4: rc = md::launch_fmt<md::NV>(format, up, dn, sms, st); break;
+        case DSL_W_MXFP4: rc = md::launch_fmt<md::MX>(format, up, dn, sms, st); break;
+        default: rc = md::launch_fmt<md::BF>(format, up, dn, sms, st); break;
     }
+    return rc != 0 ? rc : md::launch_combine(route, y, down->n, out, out_dtype, st);
 }

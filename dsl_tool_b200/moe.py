@@ -268,7 +268,7 @@ def _whole_layer(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, r
 
 def moe_decode(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, *, renormalize: bool = True,
                out_dtype=torch.float32) -> torch.Tensor:
-    """The layer for at most 32 tokens on a GPU that holds every expert, in two kernels: x [tokens, K] (float32, bfloat16 or
+    """The layer for at most 32 tokens on a GPU that holds every expert, in three kernels: x [tokens, K] (float32, bfloat16 or
     float16), logits [tokens, experts] (float32 or bfloat16) -> [tokens, D] (float32 or bfloat16).
 
     Where `moe_forward` quantises the activations for the grouped GEMMs, here they stay as they are (weight-only quantisation):
@@ -276,7 +276,8 @@ def moe_decode(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, *, 
     the k largest, ties to the lower index; an expert whose logit is minus infinity or NaN is never chosen, and a token left
     without any gets zeros.  Weights of every packed format ("fp8", "fp8_block128", "int8", "nvfp4", "mxfp4", "bf16") as
     `MoEWeights.pack` makes them.  Sums are fp32; a float32 x and the hidden activation are rounded to 11 bits (16 with bf16
-    weights).  The result does not depend on how many tokens share the call.  More tokens: `moe_forward`."""
+    weights), values below 2^-17 of a 16-bit x may be off by 2^-25 of its row's largest.  The same call gives the same bits; beside
+    other tokens a token's fp32 sums may be split otherwise.  More tokens: `moe_forward`."""
     gu, dn = w.gate_up, w.down
     dev = _lib.require_cuda(x, logits, gu.q, dn.q)
     if x.dim() != 2 or x.shape[1] != gu.k:

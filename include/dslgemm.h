@@ -367,9 +367,10 @@ int dsl_moe_layer(const void* x, int x_dtype, const void* logits, int logits_dty
                   float hidden_gs, void* scratch, size_t scratch_bytes, void* out, int out_dtype, uint32_t* status,
                   void* stream);
 /*
- * The layer for a few tokens in two kernels, activations unquantised: route, gate/up with SwiGLU, down, combine, each chosen
- * expert's weights read once.  Weights as for dsl_moe_layer, DSL_W_INT8 too; x in any of the three types.  Rounding: weights and
- * 16-bit x exact, an fp32 x and the hidden activation to 11 bits (16 with BF16 weights), sums in fp32.  An expert whose logit is
+ * The layer for a few tokens in three kernels, activations unquantised: route, gate/up with SwiGLU, down, combine, each chosen
+ * expert's weights read once.  Weights as for dsl_moe_layer, DSL_W_INT8 too; x in any of the three types.  Rounding: weights exact,
+ * 16-bit x too (FP8, INT8, FP4 weights: values below 2^-17 to 2^-25 of their row's largest), an fp32 x and the hidden activation
+ * to 11 bits (16 with BF16 weights), sums in fp32, split the same way by the same call.  An expert whose logit is
  * minus infinity or NaN is never chosen; a token without any gets zeros.  At most DSL_MOE_DECODE_MAX_TOKENS tokens, k <= 32; K
  * and H multiples of 32 (FP4), 128 (128x128 FP8), 16 (FP8, INT8) or 8 (BF16), at most 2^20 (D: 2^18), short enough that a row fits a
  * CTA's shared memory beside the routing tables (some 36000 elements at the least); else DSL_ERR_TOO_LARGE.

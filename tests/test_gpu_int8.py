@@ -207,7 +207,8 @@ def test_moe_forward_with_int8_experts(cuda_device):
             g2 = rounded(x[t:t + 1]) @ rounded(gu[e]).t()
             h = (torch.nn.functional.silu(g2[:, :H]) * g2[:, H:]).bfloat16()
             want[t] += (wts[t, j].double() * (rounded(h) @ rounded(dn[e]).t()).bfloat16().double())[0]
-    # two bf16 roundings (2^-9 of a value each on average at most) and rare flips of an int8 rounding behind the first
+    # both sides round alike; where the last bit of an fp32 sum tips a rounding the other way, a value moves by a step (2^-7 of it in
+    # bf16, 1 / 127 of its row's largest in int8): seldom, so far less than half a bf16 step, 2^-8, over all values
     assert ((got.double() - want).norm() / want.norm()).item() < 4e-3
 
 

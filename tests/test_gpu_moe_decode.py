@@ -1,4 +1,4 @@
-"""The few-token MoE layer in two kernels against the layer in 64 bits on the packed weights' own values."""
+"""The few-token MoE layer in three kernels against the layer in 64 bits on the packed weights' own values."""
 import numpy as np
 import pytest
 import torch
@@ -194,7 +194,7 @@ def test_scale_of_the_rows(cuda_device, fmt, scale):
 
 
 def test_mxfp4_scales_far_apart(cuda_device):
-    """Blocks 2^-40 to 2^30 beside one another in a row: taken relative to the largest of a chunk, what is lost lies 2^-24 below it."""
+    """Blocks 2^-40 to 2^30 beside one another in a row: each block's sum meets its scale in fp32."""
     from dsl_tool_b200 import moe_decode
     x, logits, w = make(5, 3, 512, 128, 128, "mxfp4")
     g = torch.Generator(device="cuda").manual_seed(5)

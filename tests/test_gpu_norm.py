@@ -157,7 +157,8 @@ def test_block_of_projections(cuda_device, rows, format):
     assert torch.equal(qa, q) and torch.equal(sa, s) and torch.equal(ta, t)
     qb, sb, tb = apart(o, t)
     assert torch.equal(qb, q2) and torch.equal(sb, s2) and torch.equal(tb, t2)
-    # the product of quantised rows is what the values multiply to (fp32 sums of 512 products, bf16 result: half a step 2^-9)
+    # the product of quantised rows is what the values multiply to: fp32 sums of 512 products, and a bf16 result, of which each
+    # element is off by half a step, 2^-8 of its value at most (8 bits: a step is 2^-7 of the power of two below), so their norm too
     values = q.view(torch.int8).double() * s.double()[:, None] if format == "int8" else \
         q.view(torch.float8_e4m3fn).double() * (s.double() if format == "fp8" else s.double().repeat_interleave(128, 1))
     uv = up.q.double() * up.scale.double()[:, None] if format == "int8" else \
@@ -165,7 +166,7 @@ def test_block_of_projections(cuda_device, rows, format):
                                                    up.scale.double()[0].repeat_interleave(128, 0).repeat_interleave(128, 1))
     g = values @ uv.t()
     want = torch.nn.functional.silu(g[:, 0::2]) * g[:, 1::2]
-    assert ((h.double() - want).norm() / want.norm()).item() <= 2.0 ** -9 + 2e-5
+    assert ((h.double() - want).norm() / want.norm()).item() <= 2.0 ** -8 + 2e-5
 
 
 def test_captured_chain(cuda_device):
