@@ -1096,7 +1096,8 @@ extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, in
     if (format == DSL_W_NVFP4 && (gate_up->global_scale == nullptr || down->global_scale == nullptr)) return DSL_ERR_NULL;
     const uintptr_t vectors = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gate_up->q) | reinterpret_cast<uintptr_t>(down->q);
     const uintptr_t words = reinterpret_cast<uintptr_t>(gate_up->scale) | reinterpret_cast<uintptr_t>(down->scale);
-    if ((vectors & 15u) != 0 || (words & 3u) != 0 || (reinterpret_cast<uintptr_t>(scratch) & 255u) != 0) return DSL_ERR_ALIGN;
+    const unsigned table = format == DSL_W_NVFP4 || format == DSL_W_MXFP4 ? 15u : 3u;      // FP4: 16 scale bytes at a time
+    if ((vectors & 15u) != 0 || (words & table) != 0 || (reinterpret_cast<uintptr_t>(scratch) & 255u) != 0) return DSL_ERR_ALIGN;
     if (scratch_bytes < dsl_moe_decode_scratch_bytes(gate_up, down, tokens, k, x_dtype)) return DSL_ERR_TOO_LARGE;
     md::Args up = md::side(gate_up, tokens, k, x_dtype), dn = md::side(down, tokens, k, DSL_F32);
     const size_t entries = static_cast<size_t>(tokens) * k;

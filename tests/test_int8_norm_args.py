@@ -139,3 +139,15 @@ def test_moe_decode_arguments(cdll):
     for K in (36000, 32768):
         assert need(weight(_lib.W_BF16, 64, K), weight(_lib.W_BF16, 40, 32), tokens=1, x_dtype=_lib.F32) > 0
     del keep
+
+
+@pytest.mark.parametrize("fmt, apart", [(_lib.W_NVFP4, 4), (_lib.W_MXFP4, 8), (_lib.W_FP8_BLOCK128, 2), (_lib.W_INT8, 2)])
+def test_moe_decode_refuses_scales_that_it_cannot_load_whole(cdll, fmt, apart):
+    """FP4 scale bytes are read 16 at a time, the other formats' scales as fp32 words."""
+    keep, p = _buffer()
+    for side in range(2):
+        gu, dn = _lib.Weight(), _lib.Weight()
+        for i, (w, n, k) in enumerate(((gu, 512, 128), (dn, 40, 256))):
+            w.format, w.groups, w.n, w.k, w.q, w.scale, w.global_scale = fmt, 4, n, k, p, p + (apart if i == side else 0), p
+        assert cdll.dsl_moe_decode(p, _lib.BF16, p, 0, 2, 2, 1, ctypes.byref(gu), ctypes.byref(dn), p, 1 << 30, p, 0, None) == -3
+    del keep
