@@ -182,9 +182,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def stream_ptr(index: Optional[int] = None) -> int:
     """Handle of the current stream of device `index` (default: the current device)."""
-    if _raw_stream is None:
+    if index is None:
+        index = torch.cuda.current_device()
+    if _raw_stream is None or index is None:               # None: a device without a number, i.e. not a GPU
         return torch.cuda.current_stream(index).cuda_stream
-    return _raw_stream(torch.cuda.current_device() if index is None else index)
+    return _raw_stream(index)
 
 
 class on_device:
