@@ -28,6 +28,8 @@ Scalar = Union[None, float, torch.Tensor]
 
 
 def _out_dtype(name) -> torch.dtype:
+    if name is torch.float32 or name is torch.bfloat16:
+        return name
     if isinstance(name, torch.dtype):
         name = str(name).replace("torch.", "")
     try:
@@ -66,7 +68,7 @@ def _make_output(dev, M: int, nc: int, out_dtype, out_global_scale: Scalar, offs
     scale [1]) - exactly what quantize_fp4(result, "nvfp4", global_scale=...) would give - ready to be the A
     operand of the next FP4 GEMM."""
     if not _is_nvfp4_out(out_dtype):
-        out = torch.empty((M, nc), dtype=_out_dtype(out_dtype), device=dev)
+        out = torch.empty_strided((M, nc), (nc, 1), dtype=_out_dtype(out_dtype), device=dev)      # at two thirds of torch.empty's host time
         ep.out_dtype = _lib.F32 if out.dtype == torch.float32 else _lib.BF16
         return out, nc, out
     if out_global_scale is None:
@@ -95,18 +97,16 @@ def _epilogue(dev, scale_a: Scalar, scale_b: Scalar, out: torch.dtype,
     ep = _lib.Epilogue()
     ep.b_is_static = 1 if b_static else 0
     ep.activation = _activation_code(activation)
+    ep.scale_a_host = ep.scale_b_host = 1.0
     for name, s in (("a", scale_a), ("b", scale_b)):
-        host, devp = 1.0, None
         if isinstance(s, torch.Tensor):
             t = s.detach().to(device=dev, dtype=torch.float32).reshape(-1)
             if t.numel() != 1:
                 raise ValueError(f"scale_{name} must be a scalar")
             keep.append(t)
-            devp = t.data_ptr()
+            setattr(ep, f"scale_{name}_dev", t.data_ptr())
         elif s is not None:
-            host = float(s)
-        setattr(ep, f"scale_{name}_host", host)
-        setattr(ep, f"scale_{name}_dev", devp)
+            setattr(ep, f"scale_{name}_host", float(s))
     for name, t in (("row_scale", row_scale), ("col_scale", col_scale)):
         if t is not None:
             t = t.detach().to(device=dev, dtype=torch.float32).contiguous()
@@ -116,13 +116,27 @@ def _epilogue(dev, scale_a: Scalar, scale_b: Scalar, out: torch.dtype,
     return ep
 
 
+_ws_needs: dict = {}
+
+
+def _workspace_need(dev, problem: tuple) -> int:
+    """dsl_workspace_bytes of the current device, which is `dev`; a problem's sizes are asked for once (a microsecond a call)."""
+    key = (dev.index, problem)
+    need = _ws_needs.get(key)
+    if need is None:
+        need = int(_lib.lib().dsl_workspace_bytes(*problem))
+        if len(_ws_needs) < 4096:
+            _ws_needs[key] = need
+    return need
+
+
 def _run(dev, ep: "_lib.Epilogue", problem: tuple, launch) -> int:
     """One GEMM entry point: `launch(status, stream)` -> return code.  `problem` = (DSL_OP_* code, M, N, K, groups): the
     scratch that the kernels can use for it (dsl_workspace_bytes) is the current stream's, and its lock is held over
     the call, whose launches hand sums to one another through it."""
     with _lib.on_device(dev):
         status, stream = _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev.index)
-        need = int(_lib.lib().dsl_workspace_bytes(*problem))
+        need = _workspace_need(dev, problem)
         if need <= 0:
             return launch(status, stream)
         scratch, capturing = _lib.act_arena(dev, stream), torch.cuda.is_current_stream_capturing()
@@ -404,7 +418,7 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
         torch.cuda.set_device(dev)
     try:
         # row groups never use a workspace; the library says what a dense problem can use
-        ws_need = int(lib.dsl_workspace_bytes(_OP_OF_FORMAT[w.format], M, w.n, w.k, 1)) if groups == 1 else 0
+        ws_need = _workspace_need(dev, (_OP_OF_FORMAT[w.format], M, w.n, w.k, 1)) if groups == 1 else 0
         out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
         need = w._scratch_need.get(M)
         if need is None:
@@ -447,7 +461,8 @@ def _linear_quantized(a: torch.Tensor, act_scale: torch.Tensor, w: PackedWeight,
     if act_scale.numel() != want:
         raise ValueError(f"act_scale must hold {want} values for {M} rows of {fmt}, got {tuple(act_scale.shape)}")
     a = a.contiguous()
-    act_scale = act_scale.detach().to(torch.float32).contiguous()
+    if act_scale.dtype is not torch.float32 or not act_scale.is_contiguous():
+        act_scale = act_scale.detach().to(torch.float32).contiguous()
     offs = None
     if expert_offsets is not None:
         offs, groups = _offsets_arg(expert_offsets, dev)

@@ -79,7 +79,7 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     x = _as_2d(x)
     rows, cols = x.shape
     _check_row_cols(cols)
-    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+    q = torch.empty_like(x, dtype=torch.int8)
     s = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows == 0:                       # an empty tensor has no address
         return q, s
