@@ -36,7 +36,7 @@
 // passes on.  All sums are fp32.
 //
 // Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us (share of the rate at which the chosen experts' bytes can be
-// copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 150 (84 %); 16 tokens NVFP4 129 (73 %).
+// copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 145 (86 %); 16 tokens NVFP4 129 (73 %).
 // 8 experts, top 2, H = 14336, 3 tokens BF16 294 (85 %).  What is left: about 18 us of a layer in which nothing streams (a kernel's
 // start, routing and list 4 us and the first rows 2 us, of up and of down; the last sums), and CTAs that wait for the slowest.
 #include <cuda_bf16.h>
@@ -55,7 +55,8 @@ namespace md {
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int COMBINE_THREADS = 128;
-constexpr int SUM_PITCH = 36;            // a tile's sums: a column of 32 rows for each activation row (36: no bank conflicts)
+constexpr int SUM_PLACE = 36;            // the sums of a tile's 32 rows with one row of the activations
+constexpr int SUM_COLUMN = 3 * WARPS * SUM_PLACE + 4;      // three places a warp; the next activation row's (no bank conflicts: 4 mod 16)
 constexpr int STEP = 64;                 // bytes of a weight row that a warp takes at once
 constexpr int AHEAD = 3;                 // steps that a lane has registers for: all but one in flight
 constexpr int MIN_STEPS = 4;             // of a tile (short rows: steps without bytes)
@@ -618,7 +619,7 @@ __host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) 
     l.chosen = take(a.experts * 4);
     l.base = take(a.experts * 4);
     l.misc = take(16 + 2 * 8 * 4);                                     // two numbers; amax of the rows, their inverse factors
-    l.sums = take(3 * WARPS * a.block_rows * SUM_PITCH * 4);           // a run's first piece of a tile, its last one, a whole one
+    l.sums = take(a.block_rows * SUM_COLUMN * 4);                     // a run's first piece of a tile, its last one, a whole one
     l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 128
     l.pitch = l.part_bytes * a.parts + 64;                             // two rows start half a bank round apart
     l.rows = take(0);
@@ -735,8 +736,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         clear();
         // The sums of a tile that ends, or of the piece of it that the run has, go to one of the warp's three places in shared
         // memory: 0 a tile that begins before the run, 1 one that ends behind it, 2 a whole one, which is finished at once.
-        const int sum_floats = a.block_rows * md::SUM_PITCH;
-        float* mine = s_sums + warp * (3 * sum_floats);
+        float* mine = s_sums + warp * (3 * md::SUM_PLACE);
         // Everything from here to the segment's end, for one way of forming the products (sets: 0 rows as columns, else blocks).
         auto stream = [&](auto way) {
             constexpr int SETS = decltype(way)::value;
@@ -764,12 +764,12 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 const int from = tl * a.steps, to = from + a.steps;
                 const int place = from < run0 ? 0 : (to > run1 ? 1 : 2);
                 if (place == 2) whole = tl;
-                float* d = mine + place * sum_floats + g;
+                float* d = mine + place * md::SUM_PLACE + g;
                 if constexpr (SETS == 0) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (2 * t4 < rows) d[(2 * t4) * md::SUM_PITCH + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2];
-                        if (2 * t4 + 1 < rows) d[(2 * t4 + 1) * md::SUM_PITCH + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2 + 1];
+                        if (2 * t4 < rows) d[(2 * t4) * md::SUM_COLUMN + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2];
+                        if (2 * t4 + 1 < rows) d[(2 * t4 + 1) * md::SUM_COLUMN + 8 * j] = acc[(j >> 1) * 4 + (j & 1) * 2 + 1];
                     }
                 } else {
 #pragma unroll
@@ -782,9 +782,9 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                             if (FMT == md::NV) v[j] += __shfl_xor_sync(0xFFFFFFFFu, v[j], 2);
                         }
                         if (FMT == md::NV) {             // lane t has row j = t to write, of column k
-                            d[k * md::SUM_PITCH + 8 * t4] = t4 == 0 ? v[0] : (t4 == 1 ? v[1] : (t4 == 2 ? v[2] : v[3]));
+                            d[k * md::SUM_COLUMN + 8 * t4] = t4 == 0 ? v[0] : (t4 == 1 ? v[1] : (t4 == 2 ? v[2] : v[3]));
                         } else {                         // rows t % 2 * 2 and + 1, of column 2 k + t / 2
-                            float* e = d + (2 * k + (t4 >> 1)) * md::SUM_PITCH + 16 * (t4 & 1);
+                            float* e = d + (2 * k + (t4 >> 1)) * md::SUM_COLUMN + 16 * (t4 & 1);
                             if (2 * k + (t4 >> 1) < rows) {
                                 e[0] = t4 & 1 ? v[2] : v[0];
                                 e[8] = t4 & 1 ? v[3] : v[1];
@@ -838,10 +838,10 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 if (FMT == md::I8) common = ours ? __ldg(reinterpret_cast<const float*>(a.scale) + static_cast<size_t>(expert) * a.n + r) : 0.f;
 #pragma unroll 1
                 for (int c = 0; c < rows; ++c) {
-                    float v = mine[place * sum_floats + c * md::SUM_PITCH + lane];
+                    float v = mine[place * md::SUM_PLACE + c * md::SUM_COLUMN + lane];
 #pragma unroll 1
                     for (int w = warp + 1; w < others; ++w)
-                        if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * sum_floats) + c * md::SUM_PITCH + lane];      // (not of an empty run)
+                        if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * md::SUM_PLACE) + c * md::SUM_COLUMN + lane];      // (not of an empty run)
                     v = v * s_inverse[c] * common;
                     const int entry = plan.order[first + c];
                     if (DOWN) {
