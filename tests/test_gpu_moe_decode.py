@@ -310,3 +310,34 @@ def test_refusals(cuda_device):
         x2, l2, w2 = make(1, 2, 65536, 32, 16, "bf16", dtype=torch.float32)
         moe_decode(x2, l2, w2, 1)
     assert moe_decode(x[:0], logits[:0], w, 2).shape == (0, 128)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "nvfp4", "mxfp4"])
+def test_most_tokens_experts_and_slots(cuda_device, fmt):
+    """32 tokens that choose 32 of 1024 experts each: 1024 entries, hundreds of experts with one or a few rows."""
+    from dsl_tool_b200 import moe_decode
+    x, logits, w = make(32, 1024, 128, 32, 24, fmt)
+    got = moe_decode(x, logits, w, 32)
+    assert far(got, layer(x, logits, w, 32)) <= bound(fmt, x.dtype)
+    assert torch.equal(moe_decode(x, logits, w, 32), got)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,k", [(32, 1), (31, 2)])
+def test_all_tokens_choose_the_same_experts(cuda_device, fmt, T, k):
+    from dsl_tool_b200 import moe_decode
+    x, logits, w = make(T, 300, 384, 128, 200, fmt)
+    logits[:, [7, 299]] += 100.0
+    assert far(moe_decode(x, logits, w, k), layer(x, logits, w, k)) <= bound(fmt, x.dtype)
+
+
+@pytest.mark.parametrize("K", [8, 72, 136])
+def test_infinite_weight_at_the_end_of_a_row(cuda_device, K):
+    """What stands behind a row's end in a step of 64 bytes adds nothing to it, not the NaN that an infinity against a zero makes."""
+    from dsl_tool_b200 import moe_decode
+    x, logits, w = make(3, 2, K, 16, 24, "bf16")
+    x[:, K - 1] = x[:, K - 1].abs() + 0.5
+    w.gate_up.q[10, K - 1] = float("inf")                   # gate 5 of expert 0
+    got, want = moe_decode(x, logits, w, 2), layer(x, logits, w, 2)
+    assert torch.isinf(want).all()
+    assert torch.equal(got.double(), want)
