@@ -258,6 +258,8 @@ def gemm_int8_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, scale_a: Scalar, 
     keep: list = []
     ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation)
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+    if M == 0:
+        return ret
     rc = _run(dev, ep, (_lib.OP_GEMM_INT8, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_int8(
         qa.data_ptr(), qb_nk.data_ptr(), out.data_ptr(), ldc, M, n, K, _lib.ptr(offs), groups, ctypes.byref(ep), status, stream))
     _lib.check(rc, "dsl_gemm_int8")
@@ -420,6 +422,8 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
         # row groups never use a workspace; the library says what a dense problem can use
         ws_need = _workspace_need(dev, (_OP_OF_FORMAT[w.format], M, w.n, w.k, 1)) if groups == 1 else 0
         out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+        if M == 0:                      # an empty tensor has no address
+            return ret
         need = w._scratch_need.get(M)
         if need is None:
             need = int(lib.dsl_linear_scratch_bytes(desc.format, M, w.k, groups))
@@ -472,6 +476,8 @@ def _linear_quantized(a: torch.Tensor, act_scale: torch.Tensor, w: PackedWeight,
     keep: list = []
     ep = _epilogue(dev, None, None, None, row_scale, col_scale, keep, False, activation)
     out, ldc, ret = _make_output(dev, M, _out_cols(w.n, activation), out_dtype, out_global_scale, offs, w.groups, ep, keep)
+    if M == 0:
+        return ret
     rc = _run(dev, ep, (_OP_OF_FORMAT[fmt], M, w.n, K, w.groups), lambda status, stream: _lib.lib().dsl_linear_quantized(
         a.data_ptr(), act_scale.data_ptr(), M, ctypes.byref(desc), _lib.ptr(offs), out.data_ptr(), ldc, ctypes.byref(ep), status, stream))
     _lib.check(rc, "dsl_linear_quantized")

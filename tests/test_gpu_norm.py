@@ -188,3 +188,18 @@ def test_captured_chain(cuda_device):
         g.replay()
         want = step()
         assert all(torch.equal(i, j) for i, j in zip(out, want))
+
+
+@pytest.mark.parametrize("format", ["int8", "fp8_block128", "fp8"])
+def test_chain_of_no_rows(cuda_device, format):
+    """Nothing to do, from the norm to the projection."""
+    from dsl_tool_b200 import int8_gemm, linear, pack_weight, rms_norm
+    x, r, w = _inputs((0, 512), torch.bfloat16, torch.bfloat16)
+    packed = pack_weight(torch.randn(256, 512, device="cuda"), format, gate_up_interleave=True)
+    q, s, t = rms_norm(x, w, residual=r, format=format, scale=0.1 if format == "fp8" else None)
+    assert q.shape == (0, 512) and t.shape == (0, 512)
+    assert linear(q, packed, act_scale=s).shape == (0, 256)
+    assert linear(x, packed, activation="swiglu", out_dtype=torch.bfloat16).shape == (0, 128)
+    if format == "int8":
+        assert int8_gemm(q, packed, s).shape == (0, 256)
+        assert int8_gemm(x, torch.randn(512, 256, device="cuda")).shape == (0, 256)
