@@ -350,13 +350,36 @@ _OP_OF_FORMAT = {"fp8": _lib.OP_GEMM_FP8, "fp8_block128": _lib.OP_GEMM_FP8_GROUP
                  "mxfp4": _lib.OP_GEMM_FP4_MX, "bf16": _lib.OP_GEMM_BF16, "int8": _lib.OP_GEMM_INT8}
 
 
-def _new_weight_desc(w: PackedWeight) -> "_lib.Weight":
-    if w.format == "int8":      # read by pointer: an assembled weight has to be what pack_weight makes
-        s = w.scale
-        if w.q.dtype != torch.int8 or w.q.numel() != w.groups * w.n * w.k or not w.q.is_contiguous():
-            raise ValueError(f"an int8 weight holds contiguous int8 [{w.groups}*{w.n}, {w.k}], got {w.q.dtype} {tuple(w.q.shape)}")
-        if s is None or s.dtype != torch.float32 or s.numel() != w.groups * w.n or not s.is_contiguous() or s.device != w.q.device:
-            raise ValueError(f"an int8 weight needs {w.groups * w.n} contiguous float32 channel scales beside it")
+def _as_packed(w: PackedWeight, device: torch.device) -> bool:
+    """Whether the weight's tensors are what pack_weight makes for its format and sizes.  The calls that hand the library a dsl_weight
+    read them by pointer; anything else (assembled by hand) takes the step-by-step forms, which check or convert them, or is
+    refused.  In line and in this order because a layer of one token is bound by host time."""
+    q, scale, fmt = w.q, w.scale, w.format
+    rows, k = w.groups * w.n, w.k
+    if q.device != device or not q.is_contiguous():
+        return False
+    if fmt == "bf16":
+        return q.dtype is torch.bfloat16 and q.numel() == rows * k
+    if scale is None or scale.device != device or not scale.is_contiguous():
+        return False
+    if fmt == "int8":
+        return q.dtype is torch.int8 and q.numel() == rows * k and scale.dtype is torch.float32 and scale.numel() == rows
+    if q.dtype not in _BYTE_DTYPES:
+        return False
+    tiles = w.groups * ((w.n + 127) // 128)
+    if fmt == "fp8" or fmt == "fp8_block128":
+        return (q.numel() == rows * k and scale.dtype is torch.float32
+                and scale.numel() == (1 if fmt == "fp8" else tiles * ((k + 127) // 128)))
+    if q.numel() != rows * (k // 2) or scale.dtype not in _BYTE_DTYPES:
+        return False
+    if fmt == "mxfp4":
+        return scale.numel() >= tiles * ((k // 32 + 3) // 4) * 512
+    gs = w.global_scale
+    return (scale.numel() >= tiles * ((k // 16 + 3) // 4) * 512
+            and gs is not None and gs.dtype is torch.float32 and gs.device == device and gs.numel() == 1)
+
+
+def _desc_of(w: PackedWeight) -> "_lib.Weight":
     d = _lib.Weight()
     d.format, d.groups, d.n, d.k = _W_CODES[w.format], w.groups, w.n, w.k
     d.q = w.q.data_ptr()
@@ -365,18 +388,45 @@ def _new_weight_desc(w: PackedWeight) -> "_lib.Weight":
     return d
 
 
+def _new_weight_desc(w: PackedWeight) -> "_lib.Weight":
+    if not _as_packed(w, w.q.device):
+        raise ValueError(f"this {w.format} weight is not laid out as pack_weight makes it for {w.groups} x [{w.n}, {w.k}]: "
+                         + ", ".join(f"{name} {'missing' if t is None else f'{t.dtype} {tuple(t.shape)} on {t.device}'}"
+                                     for name, t in (("q", w.q), ("scale", w.scale), ("global_scale", w.global_scale))))
+    return _desc_of(w)
+
+
 def _weight_desc(w: PackedWeight) -> "_lib.Weight":
-    """The weight's dsl_weight struct, built once and kept on the PackedWeight (rebuilt if its tensors were swapped)."""
-    d = getattr(w, "_cdesc", None)
-    if d is None or d.q != w.q.data_ptr() or d.scale != _lib.ptr(w.scale) or d.global_scale != _lib.ptr(w.global_scale):
-        d = _new_weight_desc(w)
-        w._cdesc = d
-        w._scratch_need = {}
+    """The weight's dsl_weight struct, built once and kept on the PackedWeight.  Other tensors (another object, or another address
+    under the same one) or other sizes are looked at again."""
+    kept = getattr(w, "_cdesc", None)
+    if kept is not None:
+        d, q, scale, gs, what = kept
+        if (q is w.q and scale is w.scale and gs is w.global_scale and what == (w.format, w.groups, w.n, w.k)
+                and d.q == q.data_ptr() and d.scale == _lib.ptr(scale) and d.global_scale == _lib.ptr(gs)):
+            return d
+        w._cdesc = None
+    d = _new_weight_desc(w)
+    w._cdesc = (d, w.q, w.scale, w.global_scale, (w.format, w.groups, w.n, w.k))
+    w._scratch_need = {}
     return d
 
 
+def _weight_desc_if_packed(w: PackedWeight) -> Optional["_lib.Weight"]:
+    """_weight_desc, or None for a weight whose tensors only want converting, which the step-by-step form does.  A weight without its
+    scales is none: that form would take the products as they are."""
+    try:
+        return _weight_desc(w)
+    except ValueError:
+        if (w.format != "bf16" and w.scale is None) or (w.format == "nvfp4" and w.global_scale is None):
+            raise
+        return None
+
+
 def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional[torch.Tensor], row_scale, col_scale,
-                     activation: Optional[str], out_global_scale: Scalar, act_global_scale: Scalar = None):
+                     activation: Optional[str], out_global_scale: Scalar, act_global_scale: Scalar = None, desc: Optional["_lib.Weight"] = None):
+    """Quantise + GEMM through the single C entry point `dsl_linear`: one call into the library, the quantised
+    activations in a per-stream arena instead of fresh allocations."""
     per_token = isinstance(act_global_scale, str)
     if per_token:
         if act_global_scale != "per_token" or w.format != "nvfp4":
@@ -388,12 +438,10 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
         act_global_scale = None
     if w.format == "int8" and (row_scale is not None or col_scale is not None):
         raise ValueError("an int8 weight's scales occupy the row_scale and col_scale slots")
-    """Quantise + GEMM through the single C entry point `dsl_linear`: one call into the library, the quantised
-    activations in a per-stream arena instead of fresh allocations."""
     dev = a.device
     lib = _lib.lib()
     M = a.shape[0]
-    desc = _weight_desc(w)
+    desc = _weight_desc(w) if desc is None else desc
     groups = w.groups
     nc = _out_cols(w.n, activation)
     keep: list = []
@@ -461,8 +509,10 @@ def _linear_quantized(a: torch.Tensor, act_scale: torch.Tensor, w: PackedWeight,
     if (a.dtype != torch.int8) if fmt == "int8" else (a.dtype not in _BYTE_DTYPES):
         raise TypeError(f"act_scale says that the activations are quantised for {fmt}, but they are {a.dtype}")
     M, K = a.shape
-    want = 1 if fmt == "fp8" else M if fmt == "int8" else M * ((K + 127) // 128)
-    if act_scale.numel() != want:
+    if fmt == "fp8_block128":            # the order matters
+        if act_scale.shape != (M, (K + 127) // 128):
+            raise ValueError(f"act_scale must be [{M}, {(K + 127) // 128}] for {M} rows of {fmt}, got {tuple(act_scale.shape)}")
+    elif act_scale.numel() != (want := 1 if fmt == "fp8" else M):
         raise ValueError(f"act_scale must hold {want} values for {M} rows of {fmt}, got {tuple(act_scale.shape)}")
     a = a.contiguous()
     if act_scale.dtype is not torch.float32 or not act_scale.is_contiguous():
@@ -514,13 +564,14 @@ def linear(a: torch.Tensor, w: PackedWeight, *, out_dtype=torch.float32,
         return _linear_quantized(a, act_scale, w, out_dtype, expert_offsets, row_scale, col_scale, activation, out_global_scale,
                                  act_global_scale)
     if (a.is_cuda and a.is_contiguous() and w.q.device == a.device and (w.groups > 1) == (expert_offsets is not None)
-            and (a.dtype == torch.bfloat16 if w.format == "bf16" else a.dtype in _FLOAT_DTYPES)):
+            and (a.dtype == torch.bfloat16 if w.format == "bf16" else a.dtype in _FLOAT_DTYPES)
+            and (desc := _weight_desc_if_packed(w)) is not None):
         offs = None
         if expert_offsets is not None:
             offs, groups = _offsets_arg(expert_offsets, a.device)
             if groups != w.groups:
                 raise ValueError(f"expert_offsets describes {groups} groups, the weight holds {w.groups}")
-        return _linear_one_call(a, w, out_dtype, offs, row_scale, col_scale, activation, out_global_scale, act_global_scale)
+        return _linear_one_call(a, w, out_dtype, offs, row_scale, col_scale, activation, out_global_scale, act_global_scale, desc)
     if act_global_scale is not None and w.format != "nvfp4":
         raise ValueError("act_global_scale applies to NVFP4 weights")
     if w.format == "int8":

@@ -31,7 +31,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .gemm_kernels import _BYTE_DTYPES, _FLOAT_DTYPES, _new_weight_desc, _weight_desc, gemm_fp4_quantized, gemm_fp8_groupwise_quantized, gemm_fp8_quantized, linear
+from .gemm_kernels import _FLOAT_DTYPES, _as_packed, _desc_of, _weight_desc, gemm_fp4_quantized, gemm_fp8_groupwise_quantized, gemm_fp8_quantized, linear
 from .quantize import PackedWeight, pack_weight, quantize_fp4, quantize_fp8
 from .sharding import arrival_expert_ids, exchange_rows, expert_ranges, return_rows
 
@@ -192,34 +192,6 @@ def _experts_fp4(p: MoEPlan, packed: torch.Tensor, sf: torch.Tensor, gs, w: MoEW
                               global_scale_b=w.down.global_scale, out_dtype=torch.bfloat16, **common)
 
 
-def _as_packed(w: PackedWeight, device: torch.device) -> bool:
-    """Whether the weight's tensors are what pack_weight makes for its format and sizes.  The one-call layer reads them by
-    pointer; anything else (assembled by hand) takes the step-by-step form, which checks or converts them.  In line and in
-    this order because a layer of one token is bound by host time."""
-    q, scale, fmt = w.q, w.scale, w.format
-    rows, k = w.groups * w.n, w.k
-    if q.device != device or not q.is_contiguous():
-        return False
-    if fmt == "bf16":
-        return q.dtype is torch.bfloat16 and q.shape == (rows, k)
-    if fmt == "int8":
-        return (q.dtype is torch.int8 and q.shape == (rows, k) and scale is not None and scale.dtype is torch.float32
-                and scale.numel() == rows and scale.device == device and scale.is_contiguous())
-    if q.dtype not in _BYTE_DTYPES or scale is None or scale.device != device or not scale.is_contiguous():
-        return False
-    tiles = w.groups * ((w.n + 127) // 128)
-    if fmt == "fp8" or fmt == "fp8_block128":
-        return (q.shape == (rows, k) and scale.dtype is torch.float32
-                and scale.numel() == (1 if fmt == "fp8" else tiles * ((k + 127) // 128)))
-    if q.shape != (rows, k // 2) or scale.dtype not in _BYTE_DTYPES:
-        return False
-    if fmt == "mxfp4":
-        return scale.numel() >= tiles * ((k // 32 + 3) // 4) * 512
-    gs = w.global_scale
-    return (scale.numel() >= tiles * ((k // 16 + 3) // 4) * 512
-            and gs is not None and gs.dtype is torch.float32 and gs.device == device and gs.numel() == 1)
-
-
 def _whole_layer(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, renormalize: bool, out_dtype,
                  act_global_scale) -> Optional[torch.Tensor]:
     """The layer through the single C entry point `dsl_moe_layer` (same launches, same bits as the steps below, without
@@ -244,7 +216,7 @@ def _whole_layer(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, r
     if gu.format == "nvfp4" and act_global_scale is not None:
         act_gs = (act_global_scale.detach().to(device=dev, dtype=torch.float32).reshape(1) if isinstance(act_global_scale, torch.Tensor)
                   else torch.full((1,), float(act_global_scale), dtype=torch.float32, device=dev))
-    du, dd = _new_weight_desc(gu), _new_weight_desc(dn)
+    du, dd = _desc_of(gu), _desc_of(dn)            # looked at above
     T = x.shape[0]
     need = int(lib.dsl_moe_layer_scratch_bytes(ctypes.byref(du), ctypes.byref(dd), T, k, 1 if fused else 0))
     if need == 0:
