@@ -91,9 +91,17 @@ def _make_output(dev, M: int, nc: int, out_dtype, out_global_scale: Scalar, offs
     return out, nc, (out, sf, gs)
 
 
+def _scale_vector(t: torch.Tensor, count: int, name: str, dev) -> torch.Tensor:
+    """The kernels read `count` factors by pointer."""
+    if t.numel() < count:
+        raise ValueError(f"{name} must hold {count} values, got {tuple(t.shape)}")
+    return t.detach().to(device=dev, dtype=torch.float32).contiguous()
+
+
 def _epilogue(dev, scale_a: Scalar, scale_b: Scalar, out: torch.dtype,
               row_scale: Optional[torch.Tensor], col_scale: Optional[torch.Tensor], keep: list,
-              b_static: bool = False, activation: Optional[str] = None) -> _lib.Epilogue:
+              b_static: bool = False, activation: Optional[str] = None, *, rows: int = 0, cols: int = 0) -> _lib.Epilogue:
+    """`rows`, `cols`: how many factors row_scale (one per token) and col_scale (one per output channel of every group) hold."""
     ep = _lib.Epilogue()
     ep.b_is_static = 1 if b_static else 0
     ep.activation = _activation_code(activation)
@@ -107,9 +115,9 @@ def _epilogue(dev, scale_a: Scalar, scale_b: Scalar, out: torch.dtype,
             setattr(ep, f"scale_{name}_dev", t.data_ptr())
         elif s is not None:
             setattr(ep, f"scale_{name}_host", float(s))
-    for name, t in (("row_scale", row_scale), ("col_scale", col_scale)):
+    for name, t, count in (("row_scale", row_scale, rows), ("col_scale", col_scale, cols)):
         if t is not None:
-            t = t.detach().to(device=dev, dtype=torch.float32).contiguous()
+            t = _scale_vector(t, count, name, dev)
             keep.append(t)
             setattr(ep, name, t.data_ptr())
     ep.out_dtype = _lib.F32 if out in (None, torch.float32) else _lib.BF16
@@ -191,7 +199,7 @@ def gemm_fp8_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, scale_a: Scalar, s
         raise ValueError(f"weight must be [{groups}*{n}, {K}] K-major bytes, got {tuple(qb_nk.shape)}")
     nc = _out_cols(n, activation)
     keep: list = []
-    ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation)
+    ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation, rows=M, cols=groups * n)
     ep.b_is_kn = 1 if b_kn else 0
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
     rc = _run(dev, ep, (_lib.OP_GEMM_FP8, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_fp8(
@@ -227,7 +235,7 @@ def gemm_fp8_groupwise_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, sa: torc
     nc = _out_cols(n, activation)
     out = torch.empty((M, nc), dtype=_out_dtype(out_dtype), device=dev)
     keep: list = []
-    ep = _epilogue(dev, None, None, out.dtype, row_scale, col_scale, keep, False, activation)
+    ep = _epilogue(dev, None, None, out.dtype, row_scale, col_scale, keep, False, activation, rows=M, cols=groups * n)
     ep.b_is_kn = 1 if b_kn else 0
     rc = _run(dev, ep, (_lib.OP_GEMM_FP8_GROUPWISE, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_fp8_groupwise(
         qa.data_ptr(), qb_nk.data_ptr(), sa.data_ptr(), sb.data_ptr(), 1 if sb_block else 0, out.data_ptr(), nc, M, n, K,
@@ -256,7 +264,7 @@ def gemm_int8_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, scale_a: Scalar, 
     col_scale, scale_b = _vector_or_scalar(scale_b, groups * n, "scale_b")
     nc = _out_cols(n, activation)
     keep: list = []
-    ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation)
+    ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation, rows=M, cols=groups * n)
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
     if M == 0:
         return ret
@@ -308,7 +316,7 @@ def gemm_fp4_quantized(pa: torch.Tensor, pb_nk: torch.Tensor, sfa: torch.Tensor,
         if token_scale.numel() != M:
             raise ValueError(f"token_scale must have {M} elements, got {token_scale.numel()}")
         row_scale = token_scale
-    ep = _epilogue(dev, global_scale_a, global_scale_b, None, row_scale, col_scale, keep, b_static, activation)
+    ep = _epilogue(dev, global_scale_a, global_scale_b, None, row_scale, col_scale, keep, b_static, activation, rows=M, cols=groups * n)
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
     sfa, sfb = _bytes2d(sfa), _bytes2d(sfb)
     op = _lib.OP_GEMM_FP4_NV if fmt == _lib.FP4_NV else _lib.OP_GEMM_FP4_MX
@@ -450,10 +458,10 @@ def _linear_one_call(a: torch.Tensor, w: PackedWeight, out_dtype, offs: Optional
     ep.activation = _activation_code(activation)
     ep.act_scale_per_token = 1 if per_token else 0
     if row_scale is not None:
-        row_scale = row_scale.detach().to(device=dev, dtype=torch.float32).contiguous()
+        row_scale = _scale_vector(row_scale, M, "row_scale", dev)
         ep.row_scale = row_scale.data_ptr()
     if col_scale is not None:
-        col_scale = col_scale.detach().to(device=dev, dtype=torch.float32).contiguous()
+        col_scale = _scale_vector(col_scale, groups * w.n, "col_scale", dev)
         ep.col_scale = col_scale.data_ptr()
     if act_global_scale is not None:
         if w.format != "nvfp4":
@@ -524,7 +532,7 @@ def _linear_quantized(a: torch.Tensor, act_scale: torch.Tensor, w: PackedWeight,
             raise ValueError(f"expert_offsets describes {groups} groups, the weight holds {w.groups}")
     desc = _weight_desc(w)
     keep: list = []
-    ep = _epilogue(dev, None, None, None, row_scale, col_scale, keep, False, activation)
+    ep = _epilogue(dev, None, None, None, row_scale, col_scale, keep, False, activation, rows=M, cols=w.groups * w.n)
     out, ldc, ret = _make_output(dev, M, _out_cols(w.n, activation), out_dtype, out_global_scale, offs, w.groups, ep, keep)
     if M == 0:
         return ret

@@ -130,3 +130,26 @@ def test_refused_or_converted(cuda_device, fmt):
             linear(x, replace(w, global_scale=None))
     with pytest.raises(ValueError):
         linear(x, replace(w, q=w.q[:-1]))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp8_block128"])
+@pytest.mark.parametrize("short", ["row_scale", "col_scale"])
+def test_factors_of_the_epilogue_are_counted(fmt, short, monkeypatch):
+    """One per token, one per output channel of every group: fewer would be read past their end."""
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "lib", lambda: None)
+    monkeypatch.setattr(gemm_kernels, "_run", lambda *args: pytest.fail("launched"))
+    q, w, offs = torch.zeros((4, K), dtype=torch.uint8), packed(fmt), torch.tensor([0, 2, 4], dtype=torch.int32)
+    s = torch.ones((1,) if fmt == "fp8" else (4, K // 128))
+    count = 4 if short == "row_scale" else 2 * N
+    for factors in (torch.ones(count - 1), torch.ones(1), torch.ones(N)[:0]):
+        with pytest.raises(ValueError, match=f"{short} must hold {count} values"):
+            linear(q, w, act_scale=s, expert_offsets=offs, **{short: factors})
+        with pytest.raises(ValueError, match=f"{short} must hold {count} values"):
+            if fmt == "fp8":
+                gemm_kernels.gemm_fp8_quantized(q, w.q, 1.0, 1.0, n=N, expert_offsets=offs, **{short: factors})
+            else:
+                gemm_kernels.gemm_fp8_groupwise_quantized(q, w.q, s, w.scale, n=N, sb_block=True, expert_offsets=offs, **{short: factors})
+        with pytest.raises(ValueError, match=f"{short} must hold {count} values"):
+            gemm_kernels._linear_one_call(torch.zeros((4, K)), w, torch.float32, offs, factors if short == "row_scale" else None,
+                                          factors if short == "col_scale" else None, None, None)
