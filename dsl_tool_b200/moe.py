@@ -32,7 +32,7 @@ import torch
 
 from . import _lib
 from .gemm_kernels import _FLOAT_DTYPES, _as_packed, _desc_of, _weight_desc, gemm_fp4_quantized, gemm_fp8_groupwise_quantized, gemm_fp8_quantized, linear
-from .quantize import PackedWeight, pack_weight, quantize_fp4, quantize_fp8
+from .quantize import PackedWeight, pack_weight, quantize_fp4, quantize_fp8, quantize_int8
 from .sharding import arrival_expert_ids, exchange_rows, expert_ranges, return_rows
 
 
@@ -334,6 +334,13 @@ def moe_partial(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, *,
         h = gemm_fp8_groupwise_quantized(rows, w.gate_up.q, sa_rows, w.gate_up.scale, n=w.gate_up.n, sb_block=True,
                                          expert_offsets=offs, activation="swiglu", out_dtype=torch.bfloat16)
         y = linear(h, w.down, expert_offsets=offs, out_dtype=torch.bfloat16)     # rows are independent: unwritten ones harm nobody
+    elif fmt == "int8":
+        # a scale per token: quantised once per token, from x as it is; the int8 rows and their scales are dispatched
+        qa, sa = quantize_int8(x)
+        rows = dispatch_rows(p, qa, w.first, w.last)
+        sa_rows = dispatch_rows(p, _pad_cols(sa[:, None], 4), w.first, w.last)[:, 0].contiguous()
+        h = linear(rows, w.gate_up, act_scale=sa_rows, expert_offsets=offs, activation="swiglu", out_dtype=torch.bfloat16)
+        y = linear(h, w.down, expert_offsets=offs, out_dtype=torch.bfloat16)     # rows are independent here too
     else:
         rows = dispatch_rows(p, x.to(torch.bfloat16), w.first, w.last)
         h = linear(rows, w.gate_up, expert_offsets=offs, activation="swiglu", out_dtype=torch.bfloat16)
