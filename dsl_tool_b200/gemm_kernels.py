@@ -202,6 +202,8 @@ def gemm_fp8_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, scale_a: Scalar, s
     ep = _epilogue(dev, scale_a, scale_b, None, row_scale, col_scale, keep, b_static, activation, rows=M, cols=groups * n)
     ep.b_is_kn = 1 if b_kn else 0
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+    if M == 0:                          # an empty tensor has no address
+        return ret
     rc = _run(dev, ep, (_lib.OP_GEMM_FP8, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_fp8(
         qa.data_ptr(), qb_nk.data_ptr(), out.data_ptr(), ldc, M, n, K, _lib.ptr(offs), groups, ctypes.byref(ep), status, stream))
     _lib.check(rc, "dsl_gemm_fp8")
@@ -237,6 +239,8 @@ def gemm_fp8_groupwise_quantized(qa: torch.Tensor, qb_nk: torch.Tensor, sa: torc
     keep: list = []
     ep = _epilogue(dev, None, None, out.dtype, row_scale, col_scale, keep, False, activation, rows=M, cols=groups * n)
     ep.b_is_kn = 1 if b_kn else 0
+    if M == 0:
+        return out
     rc = _run(dev, ep, (_lib.OP_GEMM_FP8_GROUPWISE, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_fp8_groupwise(
         qa.data_ptr(), qb_nk.data_ptr(), sa.data_ptr(), sb.data_ptr(), 1 if sb_block else 0, out.data_ptr(), nc, M, n, K,
         _lib.ptr(offs), groups, ctypes.byref(ep), status, stream))
@@ -318,6 +322,8 @@ def gemm_fp4_quantized(pa: torch.Tensor, pb_nk: torch.Tensor, sfa: torch.Tensor,
         row_scale = token_scale
     ep = _epilogue(dev, global_scale_a, global_scale_b, None, row_scale, col_scale, keep, b_static, activation, rows=M, cols=groups * n)
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+    if M == 0:                          # an empty tensor has no address
+        return ret
     sfa, sfb = _bytes2d(sfa), _bytes2d(sfb)
     op = _lib.OP_GEMM_FP4_NV if fmt == _lib.FP4_NV else _lib.OP_GEMM_FP4_MX
     rc = _run(dev, ep, (op, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_fp4(
@@ -342,6 +348,8 @@ def gemm_bf16_raw(a: torch.Tensor, b_nk: torch.Tensor, *, n: int, out_dtype=torc
     ep = _epilogue(dev, scale_a, scale_b, None, None, None, keep, False, activation)
     ep.b_is_kn = 1 if b_kn else 0
     out, ldc, ret = _make_output(dev, M, nc, out_dtype, out_global_scale, offs, groups, ep, keep)
+    if M == 0:                          # an empty tensor has no address
+        return ret
     rc = _run(dev, ep, (_lib.OP_GEMM_BF16, M, n, K, groups), lambda status, stream: _lib.lib().dsl_gemm_bf16(
         a.data_ptr(), b_nk.data_ptr(), out.data_ptr(), ldc, M, n, K, _lib.ptr(offs), groups, ctypes.byref(ep), status, stream))
     _lib.check(rc, "dsl_gemm_bf16")

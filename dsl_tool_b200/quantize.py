@@ -65,6 +65,8 @@ def quantize_fp8(x: torch.Tensor, mode: str = "per_tensor",
         s = torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=dev)
     else:
         s = torch.empty(((rows + 127) // 128, (cols + 127) // 128), dtype=torch.float32, device=dev)
+    if x.numel() == 0:                  # an empty tensor has no address; the scale of nothing is that of zeros
+        return q, s if given else s.fill_(1e-12)
     rc = _with_amax_cell(dev, mode == "per_tensor" and not given, lambda cell, stream: _lib.lib().dsl_quant_fp8(
         x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, FP8_MODES[mode], s.data_ptr(), given, q.data_ptr(), cell, stream))
     _lib.check(rc, "dsl_quant_fp8")
@@ -138,6 +140,8 @@ def quantize_fp4(x: torch.Tensor, format: str = "nvfp4",
         if cols > _lib.PER_TOKEN_MAX_COLS:
             raise ValueError(f"per-token scales need rows of at most {_lib.PER_TOKEN_MAX_COLS} elements, got {cols}")
         gs = torch.empty(rows, dtype=torch.float32, device=dev)
+        if x.numel() == 0:
+            return q, sf.zero_(), gs.fill_(1.0)
         with torch.cuda.device(dev):
             rc = _lib.lib().dsl_quant_fp4_per_token(x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, gs.data_ptr(),
                                                     q.data_ptr(), sf.data_ptr(), _lib.ptr(group_offsets), groups,
@@ -154,6 +158,8 @@ def quantize_fp4(x: torch.Tensor, format: str = "nvfp4",
                   if isinstance(global_scale, torch.Tensor)
                   else torch.full((1,), float(global_scale), dtype=torch.float32, device=dev))
             given = 1
+    if x.numel() == 0:                  # as of zeros
+        return q, sf.zero_(), gs if gs is None or given else gs.fill_(1.0)
     rc = _with_amax_cell(dev, format == "nvfp4" and not given, lambda cell, stream: _lib.lib().dsl_quant_fp4(
         x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, FP4_FORMATS[format], _lib.ptr(gs), given, q.data_ptr(), sf.data_ptr(),
         _lib.ptr(group_offsets), groups, cell, stream))
