@@ -106,10 +106,10 @@ int dsl_quant_fp4_per_token(const void* x, int dtype, long long rows, long long 
 int dsl_quant_int8(const void* x, int dtype, long long rows, long long cols, float* scale_out, int8_t* q_out, void* stream) {
     if (x == nullptr || scale_out == nullptr || q_out == nullptr) return DSL_ERR_NULL;
     if (dtype < DSL_F32 || dtype > DSL_F16) return DSL_ERR_ENUM;
-    if (rows < 0 || cols < 0 || rows > 0x7FFFFFFFll || cols % 16 != 0) return DSL_ERR_SHAPE;
+    if (rows < 0 || cols <= 0 || rows > 0x7FFFFFFFll || cols % 16 != 0) return DSL_ERR_SHAPE;
     if (cols > DSL_ROW_MAX_COLS) return DSL_ERR_TOO_LARGE;
     if (!aligned16(x) || !aligned16(q_out)) return DSL_ERR_ALIGN;
-    if (rows == 0 || cols == 0) return 0;
+    if (rows == 0) return 0;
     return static_cast<int>(launch_quant_int8(x, dtype, rows, static_cast<int>(cols), scale_out, q_out, as_stream(stream)));
 }
 

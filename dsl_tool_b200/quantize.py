@@ -83,8 +83,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _check_row_cols(cols)
     q = torch.empty_like(x, dtype=torch.int8)
     s = torch.empty(rows, dtype=torch.float32, device=dev)
-    if rows == 0:                       # an empty tensor has no address
-        return q, s
+    if x.numel() == 0:                  # an empty tensor has no address; a row of nothing has the scale of zeros
+        return q, s.fill_(1e-12)
     with _lib.on_device(dev):
         rc = _lib.lib().dsl_quant_int8(x.data_ptr(), _lib.dtype_code(x.dtype), rows, cols, s.data_ptr(), q.data_ptr(),
                                        _lib.stream_ptr(dev.index))

@@ -111,7 +111,7 @@ int dsl_pack_kn(const void* w, int dtype, int groups, int K, int N, int format, 
 /*
  * int8 quantisation with one scale per row (a token of the activations, an output channel of a weight): scale_out[r] =
  * max(amax_r / 127, 1e-12), q = x / scale to the nearest whole number (ties to even; the quotient is the IEEE fp32 one).  A row
- * with a NaN gets a NaN scale.  x as for dsl_quant_fp8; cols % 16 == 0, cols <= DSL_ROW_MAX_COLS; q_out [rows, cols], 16-byte aligned.
+ * with a NaN gets a NaN scale.  x as for dsl_quant_fp8; cols % 16 == 0, 16 <= cols <= DSL_ROW_MAX_COLS; q_out [rows, cols], 16-byte aligned.
  */
 #define DSL_ROW_MAX_COLS 32768
 int dsl_quant_int8(const void* x, int dtype, long long rows, long long cols, float* scale_out, int8_t* q_out, void* stream);

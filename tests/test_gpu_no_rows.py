@@ -90,3 +90,11 @@ def test_linear_and_groups(cuda_device, fmt):
         if fmt in ("nvfp4", "fp8"):
             q, sf, gs = linear(x, one, out_dtype="nvfp4", out_global_scale=0.5)
             assert q.shape == (0, N // 2) and gs.item() == 0.5
+
+
+def test_rows_of_nothing(cuda_device):
+    """An int8 row without elements has the scale of a row of zeros."""
+    from dsl_tool_b200 import quantize_int8
+    for rows in (1, 5):
+        q, s = quantize_int8(torch.empty((rows, 0), device="cuda"))
+        assert q.shape == (rows, 0) and torch.equal(s, quantize_int8(torch.zeros((rows, 16), device="cuda"))[1])

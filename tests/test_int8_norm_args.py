@@ -151,3 +151,11 @@ def test_moe_decode_refuses_scales_that_it_cannot_load_whole(cdll, fmt, apart):
             w.format, w.groups, w.n, w.k, w.q, w.scale, w.global_scale = fmt, 4, n, k, p, p + (apart if i == side else 0), p
         assert cdll.dsl_moe_decode(p, _lib.BF16, p, 0, 2, 2, 1, ctypes.byref(gu), ctypes.byref(dn), p, 1 << 30, p, 0, None) == -3
     del keep
+
+
+def test_quant_int8_of_no_columns_is_refused(cdll):
+    """It would leave the scales unwritten."""
+    keep, p = _buffer()
+    assert cdll.dsl_quant_int8(p, 0, 4, 0, p, p, None) == -2
+    assert cdll.dsl_quant_int8(p, 0, 0, 0, p, p, None) == -2
+    del keep
