@@ -31,63 +31,71 @@ __device__ __forceinline__ void chain_link() {
 
 // ---- router: softmax over the experts, top-k ------------------------------------------------
 // One warp per token.  Ties go to the lower expert index.  weights = softmax probabilities of the
-// chosen experts, divided by their sum when `renorm` is set.
+// chosen experts, divided by their sum when `renorm` is set.  Every slot gets an expert: where a mask leaves fewer than k, minus
+// infinities follow by index, with weight 0, then NaN (whose token's weights are all NaN); all weights of a token of minus
+// infinities are 0.  So every row of the plan is written, whatever the logits.
+
+// Key of a logit: its order, NaN below minus infinity; 0 stands for "taken".
+__device__ __forceinline__ uint32_t route_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);             // one zero
+    return isnan(x) ? 1u : (b & 0x80000000u ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ float route_logit(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+// The chosen logit's softmax probability, and a probability's share of the sum.
+__device__ __forceinline__ float route_weight(float x, float mx, float sum) { return sum == 0.f ? 0.f : __fdiv_rn(expf(x - mx), sum); }
+__device__ __forceinline__ float route_share(float p, float psum) { return psum == 0.f ? 0.f : __fdiv_rn(p, psum); }
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 moe_route_kernel(const T* __restrict__ logits, int tokens, int experts, int k, int renorm, int* __restrict__ ids,
                  float* __restrict__ weights) {
     chain_link();
-    extern __shared__ float s_vals[];                     // [warps per block][experts]
+    extern __shared__ uint32_t s_keys[];                  // [warps per block][experts]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * (blockDim.x >> 5) + warp;
     if (t >= tokens) return;
-    float* v = s_vals + warp * experts;
+    uint32_t* v = s_keys + warp * experts;                // a lane's own places alone: e = lane, lane + 32, ...
     float mx = -FLT_MAX;
     for (int e = lane; e < experts; e += 32) {
         float x;
         if (sizeof(T) == 4) x = reinterpret_cast<const float*>(logits)[static_cast<size_t>(t) * experts + e];
         else x = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(logits)[static_cast<size_t>(t) * experts + e]);
-        v[e] = x;
+        v[e] = route_key(x);
         mx = fmaxf(mx, x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     float sum = 0.f;
-    for (int e = lane; e < experts; e += 32) sum += expf(v[e] - mx);
+    for (int e = lane; e < experts; e += 32) sum += expf(route_logit(v[e]) - mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    __syncwarp();
     float chosen_p = 0.f;       // lane j keeps the j-th choice (k <= 32)
     int chosen_e = 0;
     float psum = 0.f;
     for (int j = 0; j < k; ++j) {
-        float best = -FLT_MAX;
+        uint32_t best = 0u;
         int bi = 0x7FFFFFFF;
         for (int e = lane; e < experts; e += 32) {
-            const float x = v[e];
+            const uint32_t x = v[e];
             if (x > best) { best = x; bi = e; }           // ascending e: the first maximum wins inside a lane
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-            const int oi = __shfl_xor_sync(0xFFFFFFFFu, bi, o);
-            if (ob > best || (ob == best && oi < bi)) { best = ob; bi = oi; }
-        }
-        const float p = __fdiv_rn(expf(best - mx), sum);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);      // not 0: k <= experts
+        bi = __reduce_min_sync(0xFFFFFFFFu, best == top ? bi : 0x7FFFFFFF);
+        const float p = route_weight(route_logit(top), mx, sum);
         psum += p;
         if (lane == j) { chosen_p = p; chosen_e = bi; }
-        if (lane == (bi & 31)) v[bi] = -FLT_MAX;
-        __syncwarp();
+        if (lane == (bi & 31)) v[bi] = 0u;
     }
     if (lane < k) {
         ids[static_cast<size_t>(t) * k + lane] = chosen_e;
-        weights[static_cast<size_t>(t) * k + lane] = renorm ? __fdiv_rn(chosen_p, psum) : chosen_p;
+        weights[static_cast<size_t>(t) * k + lane] = renorm ? route_share(chosen_p, psum) : chosen_p;
     }
 }
 
 // The same router for up to 64 experts with the logits in registers (lane l holds experts l and l + 32): no shared
-// memory, no warp barrier per round.  Every sum, comparison and division is the one of the kernel above, in the same
-// order, so ids and weights are bit-identical; the shared-memory form issued 1160 instructions per token.
+// memory.  Every sum, comparison and division is the one of the kernel above, in the same order, so ids and weights are
+// bit-identical.
 template <typename T>
 __global__ void __launch_bounds__(256)
 moe_route64_kernel(const T* __restrict__ logits, int tokens, int experts, int k, int renorm, int* __restrict__ ids,
@@ -97,50 +105,44 @@ moe_route64_kernel(const T* __restrict__ logits, int tokens, int experts, int k,
     const int t = blockIdx.x * (blockDim.x >> 5) + warp;
     if (t >= tokens) return;
     const bool has0 = lane < experts, has1 = lane + 32 < experts;
-    float v0 = -FLT_MAX, v1 = -FLT_MAX;
+    float x0 = -FLT_MAX, x1 = -FLT_MAX;
     if (sizeof(T) == 4) {
         const float* row = reinterpret_cast<const float*>(logits) + static_cast<size_t>(t) * experts;
-        if (has0) v0 = row[lane];
-        if (has1) v1 = row[lane + 32];
+        if (has0) x0 = row[lane];
+        if (has1) x1 = row[lane + 32];
     } else {
         const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(logits) + static_cast<size_t>(t) * experts;
-        if (has0) v0 = __bfloat162float(row[lane]);
-        if (has1) v1 = __bfloat162float(row[lane + 32]);
+        if (has0) x0 = __bfloat162float(row[lane]);
+        if (has1) x1 = __bfloat162float(row[lane + 32]);
     }
     float mx = -FLT_MAX;
-    if (has0) mx = fmaxf(mx, v0);
-    if (has1) mx = fmaxf(mx, v1);
+    if (has0) mx = fmaxf(mx, x0);
+    if (has1) mx = fmaxf(mx, x1);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     float sum = 0.f;
-    if (has0) sum += expf(v0 - mx);
-    if (has1) sum += expf(v1 - mx);
+    if (has0) sum += expf(x0 - mx);
+    if (has1) sum += expf(x1 - mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    uint32_t v0 = has0 ? route_key(x0) : 0u, v1 = has1 ? route_key(x1) : 0u;
     float chosen_p = 0.f;
     int chosen_e = 0;
     float psum = 0.f;
     for (int j = 0; j < k; ++j) {
-        float best = -FLT_MAX;
-        int bi = 0x7FFFFFFF;
-        if (has0 && v0 > best) { best = v0; bi = lane; }
-        if (has1 && v1 > best) { best = v1; bi = lane + 32; }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-            const int oi = __shfl_xor_sync(0xFFFFFFFFu, bi, o);
-            if (ob > best || (ob == best && oi < bi)) { best = ob; bi = oi; }
-        }
-        const float p = __fdiv_rn(expf(best - mx), sum);
+        const uint32_t best = max(v0, v1);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        const int bi = __reduce_min_sync(0xFFFFFFFFu, best != top ? 0x7FFFFFFF : (v0 == top ? lane : lane + 32));
+        const float p = route_weight(route_logit(top), mx, sum);
         psum += p;
         if (lane == j) { chosen_p = p; chosen_e = bi; }
         if (lane == (bi & 31)) {
-            if (bi < 32) v0 = -FLT_MAX; else v1 = -FLT_MAX;
+            if (bi < 32) v0 = 0u; else v1 = 0u;
         }
     }
     if (lane < k) {
         ids[static_cast<size_t>(t) * k + lane] = chosen_e;
-        weights[static_cast<size_t>(t) * k + lane] = renorm ? __fdiv_rn(chosen_p, psum) : chosen_p;
+        weights[static_cast<size_t>(t) * k + lane] = renorm ? route_share(chosen_p, psum) : chosen_p;
     }
 }
 
@@ -234,7 +236,7 @@ moe_place_kernel(const int* __restrict__ ids, int entries, int experts, const in
         const int i = c0 + threadIdx.x;
         const bool valid = i < entries;
         int e = valid ? ids[i] : -1;
-        if (e < 0 || e >= experts) e = -1;                 // out-of-range ids get no row
+        if (e < 0 || e >= experts) e = -1;                 // out-of-range ids get no row: -1
         const unsigned peers = __match_any_sync(0xFFFFFFFFu, e);
         const int rank = __popc(peers & ((1u << lane) - 1u));
         const int leader = __ffs(peers) - 1;
@@ -246,7 +248,7 @@ moe_place_kernel(const int* __restrict__ ids, int entries, int experts, const in
                     s_next[e] = base + __popc(peers);
                 }
                 base = __shfl_sync(0xFFFFFFFFu, base, leader);
-                if (e >= 0) dest[i] = base + rank;
+                if (valid) dest[i] = e >= 0 ? base + rank : -1;
             }
             __syncthreads();
         }
@@ -294,6 +296,7 @@ moe_pack_wire_fp4_kernel(const uint8_t* __restrict__ q_in, const uint8_t* __rest
     const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= entries) return;
+    if (dest[i] < 0) return;                                // an id without an expert has no record
     const int t = i / k;
     const uint4* src = reinterpret_cast<const uint4*>(q_in + static_cast<size_t>(t) * row_bytes);
     uint8_t* rec = wire + static_cast<size_t>(dest[i]) * wire_bytes;

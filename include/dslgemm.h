@@ -316,10 +316,12 @@ int dsl_gemm_fp4_ref32(const uint8_t* A, const uint8_t* B, float* C, const float
  * Mixture-of-experts steps either side of the grouped GEMM (the reference stops at the grouped GEMM itself,
  * cuda/gemm/grouped_gemm.cu:79-104; these have no counterpart there).  All deterministic.
  *   dsl_moe_route     logits [tokens, experts] (f32 / bf16) -> ids [tokens, k] (int32, ties to the lower index) and
- *                     weights [tokens, k] = softmax probabilities of the chosen experts (renorm: divided by their sum)
+ *                     weights [tokens, k] = softmax probabilities of the chosen experts (renorm: divided by their sum).
+ *                     Where a mask leaves fewer than k, minus infinities follow in index order with weight 0, then NaN (the
+ *                     weights of a token with a NaN are NaN); a token of minus infinities alone has weights 0
  *   dsl_moe_plan      ids -> offsets [experts+1] (rows per expert, prefix sums: the group_offsets of the GEMMs),
  *                     tile0 [experts+1] (prefix sums of ceil(rows/128): first scale tile of each expert) and
- *                     dest [tokens*k]: row of entry token*k+slot in the expert-sorted order (stable);
+ *                     dest [tokens*k]: row of entry token*k+slot in the expert-sorted order (stable; -1 for an id outside);
  *                     scratch: dsl_moe_plan_scratch_bytes(entries, experts) bytes
  *   dsl_moe_dispatch_fp4  copies the packed rows and scale bytes of tokens quantised ONCE (q_in [tokens, K/2], sf_in
  *                     token-major scale tiles) to their expert-sorted rows for the experts [first, last): q_out
