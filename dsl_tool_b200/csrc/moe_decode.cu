@@ -170,11 +170,11 @@ __device__ __forceinline__ int choose(const Router& r, int t, uint32_t* v, int l
 }
 
 // Weight of lane j's choice `e`: softmax over all experts, with the arithmetic of moe_route_kernel (moe.cu), so that it is
-// dsl_moe_route's.  One warp.
-__device__ __forceinline__ float weigh(const Router& r, int t, int e, int lane) {
+// dsl_moe_route's.  `sum`: the softmax's denominator, NaN where a logit of the token is.  One warp.
+__device__ __forceinline__ float weigh(const Router& r, int t, int e, int lane, float& sum) {
     const size_t row = static_cast<size_t>(t) * r.experts;
     const float own = e >= 0 ? r.at(row + e) + 0.0f : 0.f, mx = __shfl_sync(0xFFFFFFFFu, own, 0);      // the first is the largest
-    float sum = 0.f;
+    sum = 0.f;
 #pragma unroll 1
     for (int i = lane; i < r.experts; i += 32) sum += expf(r.at(row + i) - mx);
 #pragma unroll
@@ -882,11 +882,14 @@ __global__ void __launch_bounds__(md::COMBINE_THREADS) moe_decode_combine_kernel
     __shared__ uint32_t s_keys[DSL_MAX_GROUPS];
     __shared__ int s_ids[32];
     __shared__ float s_weights[32];
+    __shared__ float s_start;
     const int t = blockIdx.y, k = r.k, col = (blockIdx.x * md::COMBINE_THREADS + threadIdx.x) * 4;
     if (threadIdx.x < 32) {
         const int e = md::choose(r, t, s_keys, threadIdx.x);
         s_ids[threadIdx.x] = e;                      // slots past k: none
-        s_weights[threadIdx.x] = md::weigh(r, t, e, threadIdx.x);
+        float total;
+        s_weights[threadIdx.x] = md::weigh(r, t, e, threadIdx.x, total);
+        if (threadIdx.x == 0) s_start = 0.f * total;      // a NaN among the logits is the token's result, chosen experts or not
     }
     __syncthreads();
     griddep_wait();
@@ -894,7 +897,7 @@ __global__ void __launch_bounds__(md::COMBINE_THREADS) moe_decode_combine_kernel
     if (col >= n) return;
     const bool vec = n % 4 == 0;
     const float* row = y + static_cast<size_t>(t) * k * n + col;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[4] = {s_start, s_start, s_start, s_start};
 #pragma unroll 1
     for (int j0 = 0; j0 < k; j0 += 8) {
         float4 u[8];
