@@ -160,19 +160,20 @@ template <typename T>
 struct Raw16 {
     static constexpr int WORDS = static_cast<int>(sizeof(T)) * 4;
     uint32_t w[WORDS];
+    // Ordinary loads, past the L1: sum_out may be x or residual itself, and the non-coherent path is for memory that a kernel does
+    // not write.
     __device__ __forceinline__ void load(const T* p, bool wide) {
         if (wide) {
 #pragma unroll
-            for (int i = 0; i < WORDS; i += 8) {
-                uint32_t t[8];
-                ldg256(reinterpret_cast<const uint32_t*>(p) + i, t);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[i + j] = t[j];
-            }
+            for (int i = 0; i < WORDS; i += 8)
+                asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]),
+                               "=r"(w[i + 7])
+                             : "l"(reinterpret_cast<const uint32_t*>(p) + i));
         } else {
 #pragma unroll
             for (int i = 0; i < WORDS; i += 4) {
-                const uint4 t = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i));
+                const uint4 t = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i));
                 w[i] = t.x; w[i + 1] = t.y; w[i + 2] = t.z; w[i + 3] = t.w;
             }
         }
