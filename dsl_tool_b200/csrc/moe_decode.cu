@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
 #pragma unroll 1
                     for (int w = warp + 1; w < others; ++w)
                         if (all * w / WARPS < all * (w + 1) / WARPS) v += s_sums[w * (3 * md::SUM_PLACE) + c * md::SUM_COLUMN + lane];      // (not of an empty run)
-                    v = v * s_inverse[c] * common;
+                    v = v * common * s_inverse[c];      // in this order: the last, a power of two, leads out of the range of the sums
                     const int entry = plan.order[first + c];
                     if (DOWN) {
                         if (ours) a.y[static_cast<size_t>(entry) * a.n + r] = v;
