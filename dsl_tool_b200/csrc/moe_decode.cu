@@ -31,9 +31,14 @@
 // Rounding.  Weights are exact in the 16-bit type: E4M3, e2m1 (x UE4M3) and int8 in f16, bf16 in bf16; FP4 scales that meet the sum
 // of a block instead do so in fp32.  For f16 products a row whose largest magnitude lies in [1, 2^15) is taken as it is: 16-bit
 // values are exact down to 2^-17, off by 2^-25 at most below.  Other rows are scaled by a power of two that brings the largest just
-// under 2^15, which leaves every 16-bit value within 2^-39 of that one.  An fp32 x and the hidden activation round to 11 bits (f16),
-// or to 16 (two bf16 terms) with bf16 weights - more than the 8 bits of the bf16 hidden activation that the layer of quantised GEMMs
-// passes on.  All sums are fp32.
+// under 2^15, which leaves every 16-bit value within 2^-39 of that one.  What has more bits than one 16-bit value holds:
+//   * x in fp32: x and the hidden activation are two f16 terms each, 22 bits (values below 2^-3 to 2^-25, as above); the caller asks
+//     for fp32 by giving it, and pays for the second products: 8 tokens FP8 128x128 141 -> 146 us, INT8 143 -> 146, NVFP4 95 -> 120,
+//     one token NVFP4 33 -> 38, MXFP4 33 -> 36, 16 tokens MXFP4 129 -> 187.
+//   * x in 16 bits: the hidden activation rounds to f16's 11 bits - three more than bf16, the type that such a model's layers and the
+//     layer of quantised GEMMs pass it on in.
+//   * bf16 weights: the hidden activation, and an x that is not bf16, are two bf16 terms, 16 bits.
+// All sums are fp32.
 //
 // Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us (share of the rate at which the chosen experts' bytes can be
 // copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 145 (86 %); 16 tokens NVFP4 129 (73 %).
@@ -58,7 +63,6 @@ constexpr int COMBINE_THREADS = 128;
 constexpr int SUM_PLACE = 36;            // the sums of a tile's 32 rows with one row of the activations
 constexpr int SUM_COLUMN = 3 * WARPS * SUM_PLACE + 4;      // three places a warp; the next activation row's (no bank conflicts: 4 mod 16)
 constexpr int STEP = 64;                 // bytes of a weight row that a warp takes at once
-constexpr int AHEAD = 3;                 // steps that a lane has registers for: all but one in flight
 constexpr int MIN_STEPS = 4;             // of a tile (short rows: steps without bytes)
 
 enum { F8 = 0, F8G = 1, I8 = 2, NV = 3, MX = 4, BF = 5 };
@@ -67,10 +71,14 @@ template <int FMT>
 struct Fmt {
     static constexpr int ELEMS = FMT == NV || FMT == MX ? 32 : (FMT == BF ? 8 : 16);     // in 16 bytes
     static constexpr bool BF16 = FMT == BF;                                              // type of the products
-    static constexpr int PARTS = FMT == BF ? 2 : 1;                                      // 16-bit terms of an activation, at most
     static constexpr bool FP4 = FMT == NV || FMT == MX;
     static constexpr int ROWS = FMT == MX ? 4 : 8;       // activation rows that a CTA multiplies at a time, at most
 };
+
+// Steps that a lane has registers for: all but one in flight.  MXFP4 with two terms has two sets of sums beside them and spills with
+// three (one token 36 us a layer with two, 40 with three; 16 tokens 187 / 183).
+template <int FMT, int PARTS>
+struct Ahead { static constexpr int STEPS = FMT == MX && PARTS == 2 ? 2 : 3; };
 
 struct Router {
     const void* logits;          // [tokens, experts]
@@ -94,7 +102,7 @@ struct Args {
     int steps;                   // of a tile
     unsigned div_steps, div_grid, div_k, div_block;      // 2^32 / steps, / CTAs, / k, / block_rows: see quotient()
     int block_rows;              // rows of one expert that a CTA holds at a time
-    int parts;                   // 16-bit terms an activation (2 only with bf16 products)
+    int parts;                   // 16-bit terms an activation
     float* h;                    // up: [entries, n / 2]
     float* y;                    // down: [entries, n]
 };
@@ -388,9 +396,10 @@ __device__ __forceinline__ void widen_rows(const uint4& q0, const uint4& q1, int
 }
 
 // Sums of one step, columns = rows of the activations: acc[m * 4 ..] += weights (rows g + 64 m and g + 64 m + 32) x the rows in
-// shared memory (eight columns).  `b`: this lane's place in them.  NVFP4's scales are multiplied into the weights (exactly).
-template <int FMT>
-__device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t* b, int step, int t, int parts, int part_bytes, float (&acc)[8]) {
+// shared memory (eight columns).  `b`: this lane's place in them; a second term lies part_bytes behind the first.  NVFP4's scales are
+// multiplied into the weights (exactly).
+template <int FMT, int PARTS>
+__device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t* b, int step, int t, int part_bytes, float (&acc)[8]) {
     using F = Fmt<FMT>;
     constexpr int VECS = F::ELEMS / 8;                  // 16-byte vectors of activations against one 16-byte piece of weights
     float sum[2][4];                                    // F8G: scaled before they are added
@@ -398,9 +407,9 @@ __device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t
     if (FMT == NV) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t two = widen_e4m3(word(p.s, j) >> ((t & 1) * 16));
-            hs[j][0] = __byte_perm(two, two, 0x1010);
-            hs[j][1] = __byte_perm(two, two, 0x3232);
+            const uint32_t pair = widen_e4m3(word(p.s, j) >> ((t & 1) * 16));
+            hs[j][0] = __byte_perm(pair, pair, 0x1010);
+            hs[j][1] = __byte_perm(pair, pair, 0x3232);
         }
     }
 #pragma unroll
@@ -412,7 +421,7 @@ __device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t
         const uint8_t* at = b + (step * VECS + v) * 64;
         const uint4 x = *reinterpret_cast<const uint4*>(at);
         uint4 lo;
-        if (F::PARTS == 2 && parts == 2) lo = *reinterpret_cast<const uint4*>(at + part_bytes);
+        if (PARTS == 2) lo = *reinterpret_cast<const uint4*>(at + part_bytes);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             uint32_t a0[4], a1[4];
@@ -426,7 +435,7 @@ __device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t
             }
             mma16<F::BF16>(sum[m], a0, x.x, x.y);
             mma16<F::BF16>(sum[m], a1, x.z, x.w);
-            if (F::PARTS == 2 && parts == 2) {
+            if (PARTS == 2) {
                 mma16<F::BF16>(sum[m], a0, lo.x, lo.y);
                 mma16<F::BF16>(sum[m], a1, lo.z, lo.w);
             }
@@ -443,9 +452,11 @@ __device__ __forceinline__ void step_products(const Piece<FMT>& p, const uint8_t
 // sum and its scale meets one fp32 number instead of sixteen weights - half of the instructions that the widening above takes.
 // Lane t holds blocks 2 t and 2 t + 1, as values and as columns (NVFP4), or block t, and columns t % 2 * 2 and + 1 (MXFP4).
 // acc[set * 4 + j]: row j of the weights, of the lane's columns; a set is a row (NVFP4) or two rows (MXFP4) of the activations.
-// `b`: per set and half of a piece, this lane's place in its row or in the row of zeros.
-template <int FMT, int SETS>
-__device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* const (&b)[SETS][2], int step, int t, float (&acc)[8]) {
+// `b`: per set and half of a piece, this lane's place in its row or among the zeros of one step; `own`: all ones or zero, whether it
+// moves on with the steps and has a second term.
+template <int FMT, int SETS, int PARTS>
+__device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* const (&b)[SETS][2], const unsigned (&own)[SETS][2], int step,
+                                            int t, int part_bytes, float (&acc)[8]) {
     float sum[SETS][2][4];
 #pragma unroll
     for (int k = 0; k < SETS; ++k)
@@ -455,9 +466,14 @@ __device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* 
             for (int j = 0; j < 4; ++j) sum[k][m][j] = 0.f;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-        uint4 x[SETS];
+        uint4 x[SETS], lo[SETS];
 #pragma unroll
-        for (int k = 0; k < SETS; ++k) x[k] = *reinterpret_cast<const uint4*>(b[k][FMT == NV ? v / 2 : 0] + (step * 4 + v) * 64);
+        for (int k = 0; k < SETS; ++k) {
+            const int i = FMT == NV ? v / 2 : 0;
+            const uint8_t* at = b[k][i] + (PARTS == 2 ? static_cast<unsigned>(step * 256) & own[k][i] : step * 256) + v * 64;
+            x[k] = *reinterpret_cast<const uint4*>(at);
+            if (PARTS == 2) lo[k] = *reinterpret_cast<const uint4*>(at + (static_cast<unsigned>(part_bytes) & own[k][i]));
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             uint32_t a0[4], a1[4];
@@ -466,20 +482,24 @@ __device__ __forceinline__ void step_blocks(const Piece<FMT>& p, const uint8_t* 
             for (int k = 0; k < SETS; ++k) {
                 mma16<false>(sum[k][m], a0, x[k].x, x[k].y);
                 mma16<false>(sum[k][m], a1, x[k].z, x[k].w);
+                if (PARTS == 2) {
+                    mma16<false>(sum[k][m], a0, lo[k].x, lo[k].y);
+                    mma16<false>(sum[k][m], a1, lo[k].z, lo[k].w);
+                }
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t two = word(p.s, j) >> ((t & 1) * 16);
+        const uint32_t pair = word(p.s, j) >> ((t & 1) * 16);
         float s0, s1;
         if (FMT == NV) {
-            const uint32_t h = widen_e4m3(two);
+            const uint32_t h = widen_e4m3(pair);
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
             s0 = f.x;
             s1 = f.y;
         } else {
-            const uint32_t h = widen_ue8m0(two);
+            const uint32_t h = widen_ue8m0(pair);
             s0 = __uint_as_float(h << 16);
             s1 = __uint_as_float(h & 0xFFFF0000u);
         }
@@ -526,10 +546,14 @@ __device__ __forceinline__ float row_factor(uint32_t amax, float* inverse) {
 // 2^-25 at most below, 2^-25 of the largest.  Normed activations do.
 __device__ __forceinline__ bool fits_f16(uint32_t amax) { return amax >= __float_as_uint(1.0f) && amax < __float_as_uint(32768.0f); }
 
+// Zeros behind the rows, which FP4's columns without a value multiply: a row of them, or one step's (256 bytes) where rows of two
+// terms leave less room; there the lane's place in them does not move on with the steps.
+__host__ __device__ inline int zero_bytes(int parts, int part_bytes) { return parts == 2 ? 256 : part_bytes; }
+
 // Rows first .. first + rows of the list; element j of a row lies in step j / (4 E), lane t = j / E % 4, vector j % E / 8, i.e. at
-// ((step * E / 8 + vector) * 4 + t) * 16 bytes.  Elements past the row's end up to whole steps are zeros; with FP4 weights a row of
-// zeros follows the last one.  One look at the rows, a second one where some have to be scaled (`scaled`: they may have to be).
-template <int FMT, bool DOWN>
+// ((step * E / 8 + vector) * 4 + t) * 16 bytes.  Elements past the row's end up to whole steps are zeros; with FP4 weights
+// zeros follow the last one.  One look at the rows, a second one where some have to be scaled (`scaled`: they may have to be).
+template <int FMT, bool DOWN, int PARTS>
 __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int first, int rows, uint8_t* dst, int pitch, int part_bytes,
                                            bool scaled, uint32_t* s_amax, float* s_inverse) {
     using F = Fmt<FMT>;
@@ -568,19 +592,23 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
                 for (int i = 0; i < 4; ++i) {
                     const float f0 = f[2 * i] * factor, f1 = f[2 * i + 1] * factor;
                     m = max(m, max(__float_as_uint(f[2 * i]) & 0x7FFFFFFFu, __float_as_uint(f[2 * i + 1]) & 0x7FFFFFFFu));
+                    // the second term is the exact rest of the first, rounded; an infinity leaves none
                     if (F::BF16) {
                         const __nv_bfloat162 hi = __floats2bfloat162_rn(f0, f1);
-                        const float h0 = __low2float(hi), h1 = __high2float(hi);       // an infinity leaves no rest
+                        const float h0 = __low2float(hi), h1 = __high2float(hi);
                         const __nv_bfloat162 rest = __floats2bfloat162_rn(isinf(h0) ? 0.f : f0 - h0, isinf(h1) ? 0.f : f1 - h1);
                         w[i] = *reinterpret_cast<const uint32_t*>(&hi);
                         lo[i] = *reinterpret_cast<const uint32_t*>(&rest);
                     } else {
-                        const __half2 h = __floats2half2_rn(f0, f1);
-                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        const __half2 hi = __floats2half2_rn(f0, f1);
+                        const float h0 = __low2float(hi), h1 = __high2float(hi);
+                        const __half2 rest = __floats2half2_rn(isinf(h0) ? 0.f : f0 - h0, isinf(h1) ? 0.f : f1 - h1);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&hi);
+                        lo[i] = *reinterpret_cast<const uint32_t*>(&rest);
                     }
                 }
                 *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-                if (F::PARTS == 2 && a.parts == 2) *reinterpret_cast<uint4*>(d + part_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                if (PARTS == 2) *reinterpret_cast<uint4*>(d + part_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             if (scaled && !again) {
                 m = __reduce_max_sync(0xFFFFFFFFu, m);
@@ -589,7 +617,7 @@ __device__ __forceinline__ void stage_rows(const Args& a, const Plan& p, int fir
         }
         if (F::FP4 && !again)
 #pragma unroll 1
-            for (int v = threadIdx.x; v < part_bytes / 16; v += THREADS)
+            for (int v = threadIdx.x; v < zero_bytes(PARTS, part_bytes) / 16; v += THREADS)
                 *reinterpret_cast<uint4*>(dst + static_cast<size_t>(rows) * pitch + v * 16) = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
         if (!scaled || again) return;
@@ -623,7 +651,7 @@ __host__ __device__ inline Layout layout_of(const Args& a, int elems, bool fp4) 
     l.part_bytes = a.steps * (STEP / 16) * elems * 2;                  // a multiple of 128
     l.pitch = l.part_bytes * a.parts + 64;                             // two rows start half a bank round apart
     l.rows = take(0);
-    int room = (a.block_rows + (fp4 ? 1 : 0)) * l.pitch;
+    int room = a.block_rows * l.pitch + (fp4 ? zero_bytes(a.parts, l.part_bytes) : 0);
     if (room < WARPS * a.experts * 4) room = WARPS * a.experts * 4;
     l.total = l.rows + room;
     return l;
@@ -636,9 +664,10 @@ __device__ __forceinline__ int row_of(int tile, int g, int j) { return (tile >> 
 
 }  // namespace md
 
-template <int FMT, bool DOWN>
+template <int FMT, bool DOWN, int PARTS>
 __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Args a) {
     using F = md::Fmt<FMT>;
+    constexpr int AHEAD = md::Ahead<FMT, PARTS>::STEPS;
     using md::THREADS;
     using md::WARPS;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -692,7 +721,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         int at = run0, tile = md::quotient(run0, a.steps, a.div_steps), step = run0 - tile * a.steps;      // tile counts from tile0
 
         // Where the loads are: up to AHEAD - 1 steps before the products.
-        static_assert(md::AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
+        static_assert(AHEAD <= md::MIN_STEPS, "two tiles could end in one round of the loop below");
         int l_at = run0, l_step = step, l_tile = tile0 + tile;
         const uint8_t *l_row = nullptr, *l_scale = nullptr;
         unsigned l_rows[4] = {0u, 0u, 0u, 0u};      // from l_row to the lane's rows: where one is not there or not this CTA's, to another
@@ -706,7 +735,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
             if (FMT == md::NV || FMT == md::MX) l_scale = a.scale + block * a.katoms * 512 + ((l_tile & 3) * 8 + g) * 16;
             if (FMT == md::F8G) l_scale = a.scale + block * (a.kdim / 128) * 4;
         };
-        md::Piece<FMT> buf[md::AHEAD];
+        md::Piece<FMT> buf[AHEAD];
         auto fetch = [&](md::Piece<FMT>& p) {
             if (l_at < run1) {
                 p.load(a, l_row, l_rows, l_scale, l_step, t4);
@@ -720,14 +749,14 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
         };
         if (run0 < run1) locate();
 #pragma unroll
-        for (int i = 0; i + 1 < md::AHEAD; ++i) fetch(buf[i]);
+        for (int i = 0; i + 1 < AHEAD; ++i) fetch(buf[i]);
         if (!waited) {           // the hidden activation is up's
             griddep_wait();
             griddep_launch_dependents();
             waited = true;
         }
         __syncthreads();         // the segment before is finished, the router's room is free
-        md::stage_rows<FMT, DOWN>(a, plan, first, rows, s_rows, l.pitch, l.part_bytes, scaled, s_amax, s_inverse);
+        md::stage_rows<FMT, DOWN, PARTS>(a, plan, first, rows, s_rows, l.pitch, l.part_bytes, scaled, s_amax, s_inverse);
         float acc[8];
         auto clear = [&]() {
 #pragma unroll
@@ -742,6 +771,7 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
             constexpr int SETS = decltype(way)::value;
             constexpr int HELD = SETS > 0 ? SETS : 1;
             const uint8_t* b[HELD][2];
+            unsigned own[HELD][2];
             if (SETS == 0) {
                 b[0][0] = b[0][1] = s_rows + static_cast<size_t>(min(g, rows - 1)) * l.pitch + t4 * 16;      // columns past the rows: any
             } else {
@@ -753,11 +783,12 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                         const int r = FMT == md::NV ? k : 2 * k + (g >> 2);
                         const bool mine_too = (FMT == md::NV ? g == 2 * t4 + i : (g & 3) == t4) && r < rows;
                         b[k][i] = s_rows + static_cast<size_t>(mine_too ? r : rows) * l.pitch + t4 * 16;
+                        own[k][i] = mine_too ? ~0u : 0u;
                     }
             }
             auto multiply = [&](const md::Piece<FMT>& p) {
-                if constexpr (SETS == 0) md::step_products<FMT>(p, b[0][0], step, t4, a.parts, l.part_bytes, acc);
-                else md::step_blocks<FMT, HELD>(p, b, step, t4, acc);
+                if constexpr (SETS == 0) md::step_products<FMT, PARTS>(p, b[0][0], step, t4, l.part_bytes, acc);
+                else md::step_blocks<FMT, HELD, PARTS>(p, b, own, step, t4, l.part_bytes, acc);
             };
             int whole = -1;
             auto close = [&](int tl) {
@@ -799,9 +830,9 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
                 int place = 2, others = warp + 1;          // whose pieces make up the tile that is finished below
                 if (at < run1) {
 #pragma unroll
-                    for (int i = 0; i < md::AHEAD; ++i) {  // a tile has at least MIN_STEPS steps: at most one ends here
+                    for (int i = 0; i < AHEAD; ++i) {  // a tile has at least MIN_STEPS steps: at most one ends here
                         if (at < run1) {
-                            fetch(buf[(i + md::AHEAD - 1) % md::AHEAD]);
+                            fetch(buf[(i + AHEAD - 1) % AHEAD]);
                             multiply(buf[i]);
                             ++at;
                             const bool ends = ++step == a.steps;
@@ -972,15 +1003,15 @@ static cudaError_t prefer_l1(K kernel) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxL1);
 }
 
-template <int FMT, bool DOWN>
+template <int FMT, bool DOWN, int PARTS>
 static int launch_one(Args& a, int smem_bytes, int sms, cudaStream_t st) {
     static PerDeviceInt attr_set;   // per device; idempotent, a race here only repeats the same call
     const int dev = current_device_slot();
     if (dev < 0) return static_cast<int>(cudaErrorInvalidDevice);
     if (attr_set.v[dev].load(std::memory_order_acquire) == 0) {
-        const cudaError_t e = cudaFuncSetAttribute(moe_decode_kernel<FMT, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+        const cudaError_t e = cudaFuncSetAttribute(moe_decode_kernel<FMT, DOWN, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
         if (e != cudaSuccess) return static_cast<int>(e);
-        const cudaError_t c = prefer_l1(moe_decode_kernel<FMT, DOWN>);
+        const cudaError_t c = prefer_l1(moe_decode_kernel<FMT, DOWN, PARTS>);
         if (c != cudaSuccess) return static_cast<int>(c);
         attr_set.v[dev].store(1, std::memory_order_release);
     }
@@ -995,15 +1026,16 @@ static int launch_one(Args& a, int smem_bytes, int sms, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, moe_decode_kernel<FMT, DOWN>, a));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, moe_decode_kernel<FMT, DOWN, PARTS>, a));
 }
 
-static Args side(const dsl_weight* w, int tokens, int k, int x_dtype) {
+// One of the two products.  `x_dtype`: of the layer; the hidden activation is fp32.
+static Args side(const dsl_weight* w, bool is_down, int tokens, int k, int x_dtype) {
     Args a{};
     a.tokens = tokens;
     a.experts = w->groups;
     a.k = k;
-    a.x_dtype = x_dtype;
+    a.x_dtype = is_down ? DSL_F32 : x_dtype;
     a.w = static_cast<const uint8_t*>(w->q);
     a.scale = static_cast<const uint8_t*>(w->scale);
     a.global_scale = w->global_scale;
@@ -1012,7 +1044,8 @@ static Args side(const dsl_weight* w, int tokens, int k, int x_dtype) {
     const bool fp4 = w->format == DSL_W_NVFP4 || w->format == DSL_W_MXFP4;
     a.row_bytes = fp4 ? w->k / 2 : (w->format == DSL_W_BF16 ? 2 * w->k : w->k);
     a.katoms = fp4 ? (w->k / (w->format == DSL_W_NVFP4 ? 16 : 32) + 3) / 4 : 0;
-    a.parts = w->format == DSL_W_BF16 && x_dtype != DSL_BF16 ? 2 : 1;
+    // a layer with an fp32 x keeps its activations in two terms; bf16 products need a second one for whatever is not bf16
+    a.parts = x_dtype == DSL_F32 || (w->format == DSL_W_BF16 && a.x_dtype != DSL_BF16) ? 2 : 1;
     return a;
 }
 
@@ -1021,8 +1054,11 @@ static int launch_fmt(int format, Args& up, Args& down, int sms, cudaStream_t st
     int bytes_up = 0, bytes_down = 0;
     if (!plan_launch(up, format, &bytes_up) || !plan_launch(down, format, &bytes_down))
         return DSL_ERR_TOO_LARGE;
-    const int rc = launch_one<FMT, false>(up, bytes_up, sms, st);
-    return rc != 0 ? rc : launch_one<FMT, true>(down, bytes_down, sms, st);
+    const int rc = up.parts == 2 ? launch_one<FMT, false, 2>(up, bytes_up, sms, st) : launch_one<FMT, false, 1>(up, bytes_up, sms, st);
+    if (rc != 0) return rc;
+    if (down.parts == 2) return launch_one<FMT, true, 2>(down, bytes_down, sms, st);
+    if constexpr (FMT == BF) return DSL_ERR_ENUM;             // always two there
+    else return launch_one<FMT, true, 1>(down, bytes_down, sms, st);
 }
 
 static int launch_combine(const Router& r, const float* y, int n, void* out, int out_dtype, cudaStream_t st) {
@@ -1064,7 +1100,7 @@ static int check(const dsl_weight* gu, const dsl_weight* dn, int tokens, int k, 
     if (tokens > 0) {
         int bytes;
         for (int i = 0; i < 2; ++i) {
-            Args a = side(i == 0 ? gu : dn, tokens, k, i == 0 ? x_dtype : DSL_F32);
+            Args a = side(i == 0 ? gu : dn, i == 1, tokens, k, x_dtype);
             if (!plan_launch(a, gu->format, &bytes)) return DSL_ERR_TOO_LARGE;
         }
     }
@@ -1102,7 +1138,7 @@ extern "C" int dsl_moe_decode(const void* x, int x_dtype, const void* logits, in
     const unsigned table = format == DSL_W_NVFP4 || format == DSL_W_MXFP4 ? 15u : 3u;      // FP4: 16 scale bytes at a time
     if ((vectors & 15u) != 0 || (words & table) != 0 || (reinterpret_cast<uintptr_t>(scratch) & 255u) != 0) return DSL_ERR_ALIGN;
     if (scratch_bytes < dsl_moe_decode_scratch_bytes(gate_up, down, tokens, k, x_dtype)) return DSL_ERR_TOO_LARGE;
-    md::Args up = md::side(gate_up, tokens, k, x_dtype), dn = md::side(down, tokens, k, DSL_F32);
+    md::Args up = md::side(gate_up, false, tokens, k, x_dtype), dn = md::side(down, true, tokens, k, x_dtype);
     const size_t entries = static_cast<size_t>(tokens) * k;
     uint8_t* base = static_cast<uint8_t*>(scratch);
     float* h = reinterpret_cast<float*>(base);
