@@ -417,13 +417,13 @@ def _weight_desc(w: PackedWeight) -> "_lib.Weight":
     under the same one) or other sizes are looked at again."""
     kept = getattr(w, "_cdesc", None)
     if kept is not None:
-        d, q, scale, gs, what = kept
-        if (q is w.q and scale is w.scale and gs is w.global_scale and what == (w.format, w.groups, w.n, w.k)
-                and d.q == q.data_ptr() and d.scale == _lib.ptr(scale) and d.global_scale == _lib.ptr(gs)):
+        d, q, scale, gs, at, what = kept
+        if (q is w.q and scale is w.scale and gs is w.global_scale and at == (q.data_ptr(), _lib.ptr(scale), _lib.ptr(gs))
+                and what == (w.format, w.groups, w.n, w.k)):
             return d
         w._cdesc = None
     d = _new_weight_desc(w)
-    w._cdesc = (d, w.q, w.scale, w.global_scale, (w.format, w.groups, w.n, w.k))
+    w._cdesc = (d, w.q, w.scale, w.global_scale, (w.q.data_ptr(), _lib.ptr(w.scale), _lib.ptr(w.global_scale)), (w.format, w.groups, w.n, w.k))
     w._scratch_need = {}
     return d
 
