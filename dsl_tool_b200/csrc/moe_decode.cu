@@ -40,10 +40,11 @@
 //   * bf16 weights: the hidden activation, and an x that is not bf16, are two bf16 terms, 16 bits.
 // All sums are fp32.
 //
-// Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us (share of the rate at which the chosen experts' bytes can be
-// copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 145 (86 %); 16 tokens NVFP4 129 (73 %).
-// 8 experts, top 2, H = 14336, 3 tokens BF16 294 (85 %).  What is left: about 18 us of a layer in which nothing streams (a kernel's
-// start, routing and list 4 us and the first rows 2 us, of up and of down; the last sums), and CTAs that wait for the slowest.
+// Layer of 64 experts, top 8, K = D = 4096, H = 1536, weights cold, us a call (share of the rate at which the chosen experts' bytes
+// can be copied): one token NVFP4 34 (38 %), FP8 40 (58 %); 8 tokens NVFP4 98 (72 %), FP8 128x128 132-146 (83-90 %, by the experts
+// chosen and the GPU); 16 tokens NVFP4 129 (73 %).  8 experts, top 2, H = 14336, 3 tokens BF16 294 (85 %).  What is left: about 18 us
+// of a layer in which nothing streams (a kernel's start, routing and list 4 us and the first rows 2 us, of up and of down; the last
+// sums), and CTAs that wait for the slowest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -696,7 +697,8 @@ __global__ void __launch_bounds__(md::THREADS, 1) moe_decode_kernel(const md::Ar
     }
     // f16 rows are what they are, bf16 ones as bf16 too; the second bf16 term of an fp32 value wants room below the first
     const bool scaled = DOWN || a.x_dtype == DSL_F32 || (a.x_dtype == DSL_BF16 && !F::BF16);
-    // Down may get this far while up still runs: logits and weights were complete before up started.
+    // Down may get this far while up still runs - on an SM that up's CTA has left, since either fills the registers: logits and weights
+    // were complete before up started.
     // The list of work: every expert's units behind entry_cost places without work, so that a CTA which passes from one expert to
     // the next, and has to fetch that one's rows, is dealt less.
     int begin, end, seg0;

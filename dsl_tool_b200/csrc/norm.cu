@@ -10,7 +10,7 @@
 // q and s are those of the stand-alone quantisers on the fp32 y, bit for bit (quotients are correctly rounded).
 //
 // Bound by memory: x, r and w are read once, t, q and s written once (8192 x 8192 bf16 with residual: 470 MB, 72 us at the rate of
-// a copy, 76 measured).  One CTA takes a row and keeps it in registers, 16 consecutive elements a thread, so the three looks at it
+// a copy, 77 measured in a row of launches on the same few buffers, 83-90 a call on new ones).  One CTA takes a row and keeps it in registers, 16 consecutive elements a thread, so the three looks at it
 // (sum of squares, maximum, conversion) cost one trip to memory; a CTA has as many threads as the row has 16-element pieces (a row
 // of 4096: 256 threads), and rows beyond 1024 pieces give every thread two.  The reductions over a row are a shuffle tree and one
 // meeting in shared memory each.

@@ -246,11 +246,12 @@ def moe_decode(x: torch.Tensor, logits: torch.Tensor, w: MoEWeights, k: int, *, 
     Where `moe_forward` quantises the activations for the grouped GEMMs, here they stay as they are (weight-only quantisation):
     with a row or two for each chosen expert the layer is the reading of those experts' weights.  Routing is `route`'s: softmax,
     the k largest, ties to the lower index; an expert whose logit is minus infinity is never chosen, a token left without any gets
-    zeros, and a token with a NaN among its logits is NaN.  Weights of every packed format ("fp8", "fp8_block128", "int8", "nvfp4", "mxfp4", "bf16") as
-    `MoEWeights.pack` makes them.  Sums are fp32.  With a float32 x both x and the hidden activation keep 22 bits; with a 16-bit x,
-    which is exact (values below 2^-17 to 2^-25 of their row's largest), the hidden activation is rounded to 11; with bf16 weights
-    16 in every case.  The same call gives the same bits; beside
-    other tokens a token's fp32 sums may be split otherwise.  More tokens: `moe_forward`."""
+    zeros, and a token with a NaN among its logits is NaN.  Weights of every packed format ("fp8", "fp8_block128", "int8", "nvfp4",
+    "mxfp4", "bf16") as `MoEWeights.pack` makes them.  Sums are fp32.  With a float32 x both x and the hidden activation keep 22
+    bits; with a 16-bit x, which is exact (values below 2^-17 to 2^-25 of their row's largest), the hidden activation is rounded to
+    11; with bf16 weights 16 in every case.  The same call gives the same bits; beside other tokens a token's fp32 sums may be split
+    otherwise.  More tokens: `moe_forward`, which is also the faster one from about 16 tokens on with MXFP4 and BF16 weights (32
+    tokens, 64 experts, top 8: 149 against 201 us and 388 against 410)."""
     gu, dn = w.gate_up, w.down
     dev = _lib.require_cuda(x, logits, gu.q, dn.q)
     if x.dim() != 2 or x.shape[1] != gu.k:

@@ -14,7 +14,8 @@
  * [N, K] (or [G, N, K] for grouped GEMM).  FP4 operands hold two e2m1 values per byte,
  * low nibble = even k.  Block-scale bytes use the 512-byte tile layout
  *   tile(rt, kt) at (rt * ceil(nblk/4) + kt) * 512,  byte(r, c) at (r%32)*16 + (r/32)*4 + c
- * for 128 rows x 4 K-blocks per tile; dsl_sf_bytes() gives the buffer size.
+ * for 128 rows x 4 K-blocks per tile; dsl_sf_bytes() gives the buffer size.  Bytes of a weight's tiles that stand for no K-block are
+ * zero, as the quantisers write them (they meet zeros, and a NaN would stay one).
  */
 #ifndef DSLGEMM_H_
 #define DSLGEMM_H_
