@@ -373,10 +373,11 @@ int dsl_moe_layer(const void* x, int x_dtype, const void* logits, int logits_dty
  * The layer for a few tokens in three kernels, activations unquantised: route, gate/up with SwiGLU, down, combine, each chosen
  * expert's weights read once.  Weights as for dsl_moe_layer, DSL_W_INT8 too; x in any of the three types.  Rounding: weights exact,
  * 16-bit x too (FP8, INT8, FP4 weights: values below 2^-17 to 2^-25 of their row's largest).  With an fp32 x both x and the hidden
- * activation keep 22 bits, with a 16-bit x the hidden activation 11 (BF16 weights: 16 in every case).  Sums are fp32, split the same way by the same call.  An expert whose logit is
- * minus infinity is never chosen, a token of nothing else gets zeros, a token with a NaN among its logits NaN.  At most DSL_MOE_DECODE_MAX_TOKENS tokens, k <= 32; K
- * and H multiples of 32 (FP4), 128 (128x128 FP8), 16 (FP8, INT8) or 8 (BF16), at most 2^20 (D: 2^18), short enough that a row fits a
- * CTA's shared memory beside the routing tables (some 36000 elements at the least); else DSL_ERR_TOO_LARGE.
+ * activation keep 22 bits, with a 16-bit x the hidden activation 11 (BF16 weights: 16 in every case).  Sums are fp32, split the same
+ * way by the same call.  An expert whose logit is minus infinity is never chosen, a token of nothing else gets zeros, a token with a
+ * NaN among its logits NaN.  At most DSL_MOE_DECODE_MAX_TOKENS tokens, k <= 32; K and H multiples of 32 (FP4), 128 (128x128 FP8), 16
+ * (FP8, INT8) or 8 (BF16), at most 2^20 (D: 2^18), short enough that a row fits a CTA's shared memory beside the routing tables (some
+ * 36000 elements at the least); else DSL_ERR_TOO_LARGE.
  *   scratch     dsl_moe_decode_scratch_bytes bytes, 256-byte aligned, consumed within the call: calls issued in order on one
  *               stream may share it, calls that can overlap may not.  0 bytes: a problem that the call does not take
  */
